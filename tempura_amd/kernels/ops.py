@@ -1389,6 +1389,101 @@ def attention_rows(rows, col0: int, ctx, group: int, heads: int, kvh: int, dim: 
     return None if into is not None else out
 
 
+class SharedKeys:
+    """Which requests of a step begin with the same keys: the batch's requests in runs of ``counts[g]`` neighbours, the first
+    ``lengths[g]`` keys of every request of run g lying in the same pages (0: they share nothing).  Requests behind the last
+    run (``requests``: how many there are in all) share nothing.  Host lists; made once for as long as the runs stay as they are."""
+
+    def __init__(self, counts, lengths, device, requests: Optional[int] = None):
+        counts, lengths = [int(c) for c in counts], [int(v) for v in lengths]
+        _need(len(counts) == len(lengths), "SharedKeys: one length for every run of requests")
+        _need(all(c >= 0 for c in counts) and all(0 <= v < 2 ** 31 for v in lengths), "SharedKeys: counts and lengths must not be negative")
+        self.requests = sum(counts) if requests is None else int(requests)
+        _need(sum(counts) <= self.requests, "SharedKeys: more requests in runs than there are")
+        runs = [(c, v) for c, v in zip(counts, lengths) if c > 0]
+        left = self.requests - sum(counts)
+        if left:
+            runs.append((left, 0))
+        starts = [0]
+        for c, _ in runs:
+            starts.append(starts[-1] + c)
+        self.groups = len(runs)
+        #: the most keys that a run shares, the most requests of a run that shares keys, and how many runs do
+        self.max_keys = max((v for _, v in runs), default=0)
+        self.max_requests = max((c for c, v in runs if v), default=0)
+        self.sharing = sum(1 for _, v in runs if v)
+        data = torch.tensor(starts + [v for _, v in runs] + [v for c, v in runs for _ in range(c)], dtype=torch.int32).to(device)
+        self.starts, self.keys, self.each = data[: self.groups + 1], data[self.groups + 1: 2 * self.groups + 1], data[2 * self.groups + 1:]
+
+
+def prefix_attention_ok(dtype: torch.dtype, heads: int, kvh: int, dim: int, value_dim: int, page_size: int, max_q_len: int) -> bool:
+    """Whether ``prefix_attention`` reads shared keys once for all (else it is ``paged_attention``)."""
+    return allow_fast_attention and dtype in (torch.bfloat16, torch.float32) and dim == value_dim and dim in (32, 64, 128) and page_size >= 16 \
+        and page_size & (page_size - 1) == 0
+
+
+def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
+                     context_lens: torch.Tensor, token_req: torch.Tensor, scale: float, shared: SharedKeys, max_q_len: int, max_context_len: int,
+                     max_own_len: Optional[int] = None, num_single: Optional[int] = None, sink: Optional[torch.Tensor] = None,
+                     softcap: float = 0.0) -> torch.Tensor:
+    """``paged_attention`` (without a window) of a step whose requests begin with the same keys: the same operands and result, but the pages
+    that the requests of a run of ``shared`` have in common are read once for all of them.  Every request's block table names its shared pages
+    as well; its new tokens lie behind its shared keys.  ``max_own_len``: the most keys that a request has behind its shared ones, its
+    new tokens among them (a bound, at least the longest; None: ``max_context_len``).  Sizes that the kernel is not built for
+    (``prefix_attention_ok``), and steps without shared keys, run ``paged_attention``."""
+    if _backend is not None:
+        return _backend.prefix_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, shared, max_q_len,
+                                         max_context_len, max_own_len, num_single, sink, softcap)
+    _dev_ok(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, sink, shared.starts)
+    _need(q.dim() == 3 and k_cache.dim() == 4 and v_cache.dim() == 4, "prefix_attention: bad operand ranks")
+    n, heads, d = q.shape
+    pages, kvh, page_size, d2 = k_cache.shape
+    vd = v_cache.shape[2]
+    _need(tuple(v_cache.shape) == (pages, kvh, vd, page_size), "prefix_attention: v cache must be [pages, kv_heads, value_dim, page_size]")
+    _need(d == d2 and kvh > 0 and heads % kvh == 0, "prefix_attention: heads of q and cache differ")
+    _need(q.dtype == k_cache.dtype == v_cache.dtype, "prefix_attention: q and cache dtypes differ")
+    _need(block_tables.dim() == 2 and block_tables.dtype == torch.int32, "prefix_attention: block_tables must be int32 [r, width]")
+    r, width = block_tables.shape
+    if shared.requests != r:
+        raise KernelError(f"prefix_attention: runs of {shared.requests} requests for a batch of {r}")
+    _i32(cu_seqlens, r + 1, "cu_seqlens")
+    _i32(context_lens, r, "context_lens") if r else None
+    _i32(token_req, n, "token_req") if n else None
+    _need(n >= r and max_q_len >= 1, "prefix_attention: every request brings at least one token")
+    _need(max_context_len <= width * page_size, "prefix_attention: block table narrower than the longest context")
+    _need(shared.max_keys < max(1, max_context_len), "prefix_attention: a request's new tokens must lie behind its shared keys")
+    _need(softcap >= 0, "prefix_attention: softcap must not be negative")
+    own = int(max_context_len if max_own_len is None else max_own_len)
+    _need(0 < own <= max(1, max_context_len), "prefix_attention: max_own_len must be between 1 and the longest context")
+    if sink is not None:
+        _need(sink.dtype == torch.float32 and sink.numel() == heads, "prefix_attention: sink must be float32 [heads]")
+    if shared.max_keys == 0 or not prefix_attention_ok(q.dtype, heads, kvh, d, vd, page_size, max_q_len):
+        return paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, 0, max_q_len, max_context_len,
+                               num_single, sink=sink, softcap=softcap)
+    out = torch.empty((n, heads * vd), dtype=q.dtype, device=q.device)
+    if n == 0:
+        return out
+    group = heads // kvh
+    tiles = 1 if min(n, shared.max_requests * max_q_len) * group <= 16 else 2
+    own_tiles = 1 if max_q_len * group <= 16 else 2
+    rows = n * group // (16 * tiles) + shared.sharing
+    shared_steps, shared_parts = _prefix_parts(-(-shared.max_keys // 32), rows * kvh, 48)
+    own_steps, own_parts = _prefix_parts((own + 15 + 31) // 32, r * -(-max_q_len * group // (16 * own_tiles)) * kvh, 16)
+    scratch = torch.empty((n * heads * (shared_parts + own_parts) * (d + 2),), dtype=torch.float32, device=q.device)
+    _call("tp_prefix_attention", _ptr(q), _dt(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), width, _ptr(cu_seqlens), _ptr(context_lens),
+          _ptr(token_req), _ptr(shared.starts), _ptr(shared.keys), _ptr(shared.each), _ptr(out), _ptr(scratch), n, r, shared.groups, heads, kvh, d,
+          page_size, float(scale), float(softcap), _ptr(sink), int(max_q_len), tiles, own_tiles, rows, shared_steps, shared_parts, own_steps, own_parts,
+          _stream())
+    return out
+
+
+def _prefix_parts(steps: int, blocks: int, most: int) -> tuple:
+    """(steps of 32 keys a part, parts) of keys of ``steps`` steps that ``blocks`` blocks a part walk."""
+    want = min(most, -(-512 // blocks), max(1, steps // 8))
+    per = -(-steps // max(1, want))
+    return per, -(-steps // per)
+
+
 def swiglu(gu: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
     """[m, 2i] (gate columns then up columns) -> out_dtype [m, i]."""
     if _backend is not None:
