@@ -890,6 +890,71 @@ def linear(x, w: torch.Tensor, out_dtype: torch.dtype, residual: Optional[torch.
     return out if next_norm is None else (out, handed)
 
 
+#: the most slices that one projection's adapters have
+ADAPTER_SLICES = 8
+
+
+class Adapters:
+    """Low-rank adapters of one projection of ``n`` columns and ``k`` inputs, one in each slot: ``a`` [slots, slices * rank, k],
+    ``b`` [slots, n, rank] (both of the activations' type), ``scales`` float32 [slots].  A projection that several matrices were
+    stacked into has a pair for each of its slices: ``ends`` are the columns at which they end (None: one slice), slice i has the rows
+    i * rank .. of ``a``; ``interleaved``: two slices whose columns alternate by eights (``interleave_gate_up``).  Ranks that are no multiple
+    of 8 are padded with zeros here, once; otherwise the tensors are kept as they are, and what is written into them later counts."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, ends=None, interleaved: bool = False):
+        _dev_ok(a, b, scales)
+        _need(a.dim() == b.dim() == 3 and a.dtype == b.dtype and a.dtype in (torch.bfloat16, torch.float32),
+              "Adapters: a [slots, slices * rank, k] and b [slots, n, rank], bfloat16 or float32")
+        self.slots, self.n, rank = b.shape
+        ends = [self.n] if ends is None else [int(e) for e in ends]
+        self.slices = 2 if interleaved else len(ends)
+        _need(1 <= self.slices <= ADAPTER_SLICES, f"Adapters: one to {ADAPTER_SLICES} slices")
+        _need(self.slots > 0 and rank > 0 and self.n > 0 and a.shape[2] > 0, "Adapters: empty tensors")
+        _need(a.shape[0] == self.slots and a.shape[1] == self.slices * rank, "Adapters: a and b differ in slots or rank")
+        if interleaved:
+            _need(len(ends) == 1 and self.n % 16 == 0, "Adapters: interleaved slices are two, of a multiple of 8 columns each")
+        _need(ends[-1] == self.n and all(x < y for x, y in zip([0] + ends, ends)), "Adapters: ends must rise to the number of columns")
+        _need(scales.dtype == torch.float32 and tuple(scales.shape) == (self.slots,), "Adapters: scales must be float32 [slots]")
+        self.k, self.interleaved = a.shape[2], bool(interleaved)
+        self.rank = -(-rank // 8) * 8
+        _need(self.slices * self.rank <= 4096, "Adapters: ranks of all slices beyond 4,096")
+        if self.rank != rank or b.data_ptr() % 16:
+            wide = torch.zeros((self.slots, self.slices, self.rank, self.k), dtype=a.dtype, device=a.device)
+            wide[:, :, :rank] = a.view(self.slots, self.slices, rank, self.k)
+            a = wide.view(self.slots, -1, self.k)
+            wide = torch.zeros((self.slots, self.n, self.rank), dtype=b.dtype, device=b.device)
+            wide[:, :, :rank] = b
+            b = wide
+        self.a, self.b, self.scales = a, b, scales
+        self.ends = (ctypes.c_int * self.slices)(*(ends if not interleaved else [self.n, self.n]))
+
+    @property
+    def dtype(self):
+        return self.a.dtype
+
+
+def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, residual: Optional[torch.Tensor] = None, max_run: int = 0) -> torch.Tensor:
+    """x [m, k] @ w[n, k]^T plus, for every row t with an adapter, scales[id] * B_id (A_id x[t]); id = ``ids``[t] (int32 [m]; an id outside
+    the slots: no adapter) -> float32 [m, n], or added into ``residual`` (float32 [m, n]), which is returned.  ``w`` as for ``linear``.
+    ``max_run``: the most tokens that a request brings (0: not known)."""
+    if _backend is not None:
+        return _backend.adapter_linear(x, w, adapters, ids, residual)
+    _dev_ok(x, ids, residual)
+    _need(x.dim() == 2 and x.dtype == adapters.dtype, "adapter_linear: x must be [m, k] of the adapters' type")
+    m, k = x.shape
+    if not (k == adapters.k and w.dim() == 2 and tuple(w.shape) == (adapters.n, k)):
+        raise KernelError(f"adapter_linear: shapes {(m, k)} x {tuple(w.shape)} with adapters of {adapters.k} x {adapters.n}")
+    _need(ids.dtype == torch.int32 and ids.dim() == 1 and ids.numel() == m, "adapter_linear: ids must be int32 [m]")
+    _need(x.device == ids.device == adapters.a.device, "adapter_linear: operands on different devices")
+    y = linear(x, w, torch.float32, residual=residual)
+    if m == 0:
+        return y
+    vec = int(k % 8 == 0 and x.data_ptr() % 16 == 0 and adapters.a.data_ptr() % 16 == 0)
+    _call("tp_adapter_add", _ptr(ids), _ptr(x), _dt(x), _ptr(adapters.a), _ptr(adapters.b), _ptr(adapters.scales), _ptr(y), m, k, adapters.n,
+          adapters.slots, adapters.rank, adapters.slices, int(adapters.interleaved), adapters.ends, vec, _stream(), tag=(m, adapters.n, k))
+    return y
+
+
 #: rows handed from one product to the next with a norm between them travel k-blocked (up to 16 rows)
 handoff_blocked = True
 #: long steps may rotate and store in the projection's epilogue too (False: only the few rows of decoding)
