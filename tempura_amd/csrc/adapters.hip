@@ -90,18 +90,320 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(AdapterArgs a, int co
   }
 }
 
+// ---- many rows -------------------------------------------------------------------------------
+// Rows with the same adapter are brought together first: a unit is up to UNIT rows of one adapter, wherever they stand in the batch.
+//   plan: [0] units; [4 ..] units of four ints (slot, first place, rows, 0); then the rows by place
+// (The order of a unit's rows follows the atomics below and may change from run to run: a row's sums do not hang on its place.)
+#define AD_UNIT 64
+typedef __bf16 ad_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float ad_f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned int ad_u32x4 __attribute__((ext_vector_type(4)));
+
+// grid: one block.  LDS: two ints a slot.
+__global__ __launch_bounds__(1024) void adapter_plan_kernel(const int* __restrict__ ids, int rows, int slots, int4* __restrict__ units, int* __restrict__ order,
+                                                           int* __restrict__ n_units) {
+  extern __shared__ int count[];      // [slots] rows, then the next place of the slot; [slots] its first unit
+  int* first_unit = count + slots;
+  __shared__ int wave_rows[16], wave_units[16], base_rows, base_units;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int i = threadIdx.x; i < slots; i += 1024) count[i] = 0;
+  if (threadIdx.x == 0) base_rows = base_units = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const int s = ids[i];
+    if (s >= 0 && s < slots) atomicAdd(&count[s], 1);
+  }
+  __syncthreads();
+  for (int s0 = 0; s0 < slots; s0 += 1024) {        // running sums over the slots, 1,024 at a time
+    const int s = s0 + threadIdx.x;
+    const int c = s < slots ? count[s] : 0, u = (c + AD_UNIT - 1) / AD_UNIT;
+    int cr = c, cu = u;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int a = __shfl_up(cr, d, 64), b = __shfl_up(cu, d, 64);
+      if (lane >= d) {
+        cr += a;
+        cu += b;
+      }
+    }
+    if (lane == 63) {
+      wave_rows[wave] = cr;
+      wave_units[wave] = cu;
+    }
+    __syncthreads();
+    int at = base_rows + cr - c, unit = base_units + cu - u, all_r = 0, all_u = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) {
+        at += wave_rows[w];
+        unit += wave_units[w];
+      }
+      all_r += wave_rows[w];
+      all_u += wave_units[w];
+    }
+    for (int i = 0; i < u; ++i) units[unit + i] = make_int4(s, at + i * AD_UNIT, min(AD_UNIT, c - i * AD_UNIT), 0);
+    __syncthreads();
+    if (s < slots) count[s] = at;
+    if (threadIdx.x == 0) {
+      base_rows += all_r;
+      base_units += all_u;
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const int s = ids[i];
+    if (s >= 0 && s < slots) order[atomicAdd(&count[s], 1)] = i;
+  }
+  if (threadIdx.x == 0) *n_units = base_units;
+}
+
+// 16 bytes of a row from element k on, zeros behind its end (VEC: aligned, and the end is a multiple of the piece)
+template <typename T, bool VEC>
+__device__ inline ad_u32x4 load_piece(const T* row, int k, int K) {
+  constexpr int P = 16 / sizeof(T);
+  if constexpr (VEC) {
+    return k < K ? *(const ad_u32x4*)(row + k) : (ad_u32x4){0, 0, 0, 0};
+  } else {
+    union {
+      T e[P];
+      ad_u32x4 v;
+    } u;
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      u.e[i] = T{};
+      if (k + i < K) u.e[i] = row[k + i];
+    }
+    return u.v;
+  }
+}
+// c += a . b over the pieces' elements (16 bytes a lane: the lane's row of a, or column of b, of its quarter of the elements)
+template <typename T>
+__device__ inline void mfma_piece(const ad_u32x4& a, const ad_u32x4& b, ad_f32x4& c) {
+  if constexpr (sizeof(T) == 2) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(ad_bf16x8, a), __builtin_bit_cast(ad_bf16x8, b), c, 0, 0, 0);
+  } else {
+    const ad_f32x4 x = __builtin_bit_cast(ad_f32x4, a), y = __builtin_bit_cast(ad_f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+  }
+}
+
+// v[part, place, ranks] = A x of a unit's rows over one part of K: v^T[rank, row] = A[rank, :] . x[row, :]^T, 16 * RT ranks a block, the four waves
+// taking every fourth step of the part, added in LDS in their order.
+// grid: (units, parts, blocks of ranks)
+template <typename T, int RT, bool VEC>
+__global__ __launch_bounds__(256) void adapter_down_kernel(AdapterArgs a, const int4* __restrict__ units, const int* __restrict__ order,
+                                                           const int* __restrict__ n_units, float* __restrict__ v, int part_k) {
+  constexpr int STEP = 64 / sizeof(T);     // elements a step: four pieces of 16 bytes
+  if ((int)blockIdx.x >= *n_units) return;
+  const int4 u = units[blockIdx.x];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+  const int ranks = a.rank * a.slices, r0 = blockIdx.z * 16 * RT;
+  const int k0 = blockIdx.y * part_k, k1 = min(a.K, k0 + part_k);
+  const T* xr[4];
+  const T* ar[RT];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) xr[t] = (const T*)a.x + (size_t)order[u.y + min(t * 16 + c, u.z - 1)] * a.K;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) ar[t] = (const T*)a.a + ((size_t)u.x * ranks + min(r0 + t * 16 + c, ranks - 1)) * a.K;
+  const int tiles = (u.z + 15) >> 4;
+  ad_f32x4 acc[RT][4];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) acc[i][t] = (ad_f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int k = k0 + wave * STEP; k < k1; k += 4 * STEP) {
+    const int at = k + g * (STEP / 4);
+    ad_u32x4 xf[4], af[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) af[i] = load_piece<T, VEC>(ar[i], at, k1);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (t < tiles) xf[t] = load_piece<T, VEC>(xr[t], at, k1);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (t < tiles) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i) mfma_piece<T>(af[i], xf[t], acc[i][t]);
+      }
+  }
+  __shared__ float red[4][16 * RT][17];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if (t >= tiles) break;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) red[wave][i * 16 + 4 * g + r][c] = acc[i][t][r];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 256 * RT; e += 256) {
+      const int rank = e % (16 * RT), row = e / (16 * RT);
+      if (t * 16 + row < u.z && r0 + rank < ranks)
+        v[((size_t)blockIdx.y * a.rows + u.y + t * 16 + row) * ranks + r0 + rank] = (red[0][rank][row] + red[1][rank][row]) + (red[2][rank][row] + red[3][rank][row]);
+    }
+  }
+}
+
+// y[row, n] += scale * B[n, :] . v[row, :] of a unit's rows: y^T[n, row], 16 columns and 16 rows a tile, so that a lane has four neighbouring columns
+// of its row.  The low-rank values, the sum of their parts times the scale, go through LDS once a block: float32 as they are; for bfloat16
+// weights as three bfloat16 pieces, the leading, middle and last eight bits, whose sum is the value, so nothing is rounded (2 rank columns
+// products more on matrix cores that wait for y anyway).  Bound by reading and writing y.
+// A lane's weights of another slice than the one at hand are zero.  grid: (units, blocks of cols columns)
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a, const int4* __restrict__ units, const int* __restrict__ order,
+                                                         const int* __restrict__ n_units, const float* __restrict__ v, int parts, int cols) {
+  constexpr int P = 16 / sizeof(T), STEP = 4 * P;        // ranks a piece and a step
+  constexpr int PIECES = sizeof(T) == 2 ? 3 : 1, CHUNK = 64, STEPS = CHUNK / STEP;      // ranks at a time
+  constexpr int ROW = CHUNK * sizeof(T) + 16;            // bytes of a row in LDS, a bank group more than the values
+  if ((int)blockIdx.x >= *n_units) return;
+  const int4 u = units[blockIdx.x];
+  __shared__ __attribute__((aligned(16))) unsigned char low[PIECES][AD_UNIT * ROW];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+  const int n0 = blockIdx.y * cols, n1 = min(n0 + cols, a.N), ranks = a.rank * a.slices, tiles = (u.z + 15) >> 4;
+  const float scale = a.scale[u.x];
+  size_t yrow[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) yrow[t] = (size_t)order[u.y + min(t * 16 + c, u.z - 1)] * a.N;
+  const int s0 = a.interleaved ? 0 : slice_of(a, n0), s1 = a.interleaved ? 1 : slice_of(a, n1 - 1);
+  for (int s = s0; s <= s1; ++s) {
+    const int from = a.interleaved ? n0 : max(n0, s > 0 ? a.ends[s - 1] : 0), to = a.interleaved ? n1 : min(n1, a.ends[s]);
+    for (int j0 = 0; j0 < a.rank; j0 += CHUNK) {
+      __syncthreads();
+      for (int e = threadIdx.x; e < AD_UNIT * CHUNK; e += 256) {
+        const int row = e / CHUNK, j = e % CHUNK;
+        float sum = 0.f;
+        if (row < u.z && j0 + j < a.rank) {
+          const float* p = v + ((size_t)u.y + row) * ranks + s * a.rank + j0 + j;
+          for (int k = 0; k < parts; ++k) sum += p[(size_t)k * a.rows * ranks];
+          sum *= scale;
+        }
+        if constexpr (PIECES == 1) {
+          *(float*)(low[0] + row * ROW + j * 4) = sum;
+        } else {
+          float left = sum;
+#pragma unroll
+          for (int p = 0; p < PIECES; ++p) {
+            const unsigned bits = __builtin_bit_cast(unsigned, left) & 0xffff0000u;
+            *(uint16_t*)(low[p] + row * ROW + j * 2) = (uint16_t)(bits >> 16);
+            left -= __builtin_bit_cast(float, bits);
+            if (!(fabsf(sum) <= 3.4028234e38f)) left = 0.f;      // (infinite or no number: the first piece says it)
+          }
+        }
+      }
+      __syncthreads();
+      for (int n = (from & ~15) + wave * 32; n < to; n += 128) {
+        // 32 columns: two tiles
+        ad_f32x4 acc[2][4], old[2][4];
+        ad_u32x4 bf[2][STEPS];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int col = n + 16 * i + c;
+          const bool mine = col >= from && col < to && (!a.interleaved || ((col >> 3) & 1) == s);
+          const T* B = (const T*)a.b + ((size_t)u.x * a.N + min(col, a.N - 1)) * a.rank;
+#pragma unroll
+          for (int k = 0; k < STEPS; ++k) {
+            const int j = j0 + k * STEP + g * P;
+            bf[i][k] = mine && j < a.rank ? *(const ad_u32x4*)(B + j) : (ad_u32x4){0, 0, 0, 0};
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            acc[i][t] = (ad_f32x4){0.f, 0.f, 0.f, 0.f};
+            const int col = n + 16 * i + 4 * g;
+            if (VEC) {
+              if (t < tiles && col < a.N) old[i][t] = *(const ad_f32x4*)(a.y + yrow[t] + col);
+            } else if (t < tiles) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) old[i][t][r] = col + r < a.N ? a.y[yrow[t] + col + r] : 0.f;
+            }
+          }
+#pragma unroll
+        for (int k = 0; k < STEPS; ++k) {
+          if (j0 + k * STEP >= a.rank) break;
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (t < tiles) {
+#pragma unroll
+              for (int p = 0; p < PIECES; ++p) {
+                const ad_u32x4 lf = *(const ad_u32x4*)(low[p] + (t * 16 + c) * ROW + (k * 4 + g) * 16);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) mfma_piece<T>(bf[i][k], lf, acc[i][t]);
+              }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (t * 16 + c < u.z) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int col = n + 16 * i + 4 * g;
+              // (a tile that reaches into the columns of another wave, slice or block leaves those alone)
+              const bool all = col >= from && col + 4 <= to;
+              if (VEC && all) {
+                *(ad_f32x4*)(a.y + yrow[t] + col) = old[i][t] + acc[i][t];
+              } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (col + r >= from && col + r < to) a.y[yrow[t] + col + r] = old[i][t][r] + acc[i][t][r];
+              }
+            }
+          }
+      }
+    }
+  }
+}
+
+template <typename T, bool VEC>
+static void adapter_down(const AdapterArgs& g, dim3 grid, int rt, const int4* units, const int* order, const int* n, float* v, int part_k, hipStream_t s) {
+  if (rt == 1) adapter_down_kernel<T, 1, VEC><<<grid, 256, 0, s>>>(g, units, order, n, v, part_k);
+  else if (rt == 2) adapter_down_kernel<T, 2, VEC><<<grid, 256, 0, s>>>(g, units, order, n, v, part_k);
+  else adapter_down_kernel<T, 4, VEC><<<grid, 256, 0, s>>>(g, units, order, n, v, part_k);
+}
+
 // y [rows, N] float32 += the adapters' share.  a [slots, slices * rank, K], b [slots, N, rank] of dt, rank a multiple of 8; vec: K is a multiple of
-// 8 and x and a are aligned to 16 bytes.  ends: the columns at which the slices end (the last is N).
+// 8 and x and a are aligned to 16 bytes.  ends: the columns at which the slices end (the last is N).  parts 0: a block a row; else rows brought
+// together by adapter, K in `parts` parts, with scratch of 4 + 4 * units + rows ints (units: rows / 64 + the smaller of slots and rows), rounded up to
+// a multiple of 4, and parts * rows * slices * rank floats behind them.
 extern "C" int tp_adapter_add(const int* ids, const void* x, int dt, const void* a, const void* b, const float* scale, float* y, int rows, int K, int N,
-                              int slots, int rank, int slices, int interleaved, const int* ends, int vec, hipStream_t s) {
+                              int slots, int rank, int slices, int interleaved, const int* ends, int vec, int parts, void* scratch, hipStream_t s) {
   if (rows <= 0 || N <= 0) return 0;
   TP_REQUIRE(dt == TP_BF16 || dt == TP_F32, "adapter_add: unsupported element type");
   TP_REQUIRE(K > 0 && slots > 0 && rank > 0 && rank % 8 == 0 && slices >= 1 && slices <= AD_MAX_SLICES, "adapter_add: bad sizes");
   TP_REQUIRE(!interleaved || (slices == 2 && N % 16 == 0), "adapter_add: two interleaved slices");
-  TP_REQUIRE(rows <= 65535, "adapter_add: too many rows");
   AdapterArgs g = {ids, x, a, b, scale, y, rows, K, N, slots, rank, slices, interleaved, {}};
   for (int i = 0; i < slices; ++i) g.ends[i] = ends[i];
+  if (parts > 0) {
+    TP_REQUIRE(scratch != nullptr && slots <= 4096, "adapter_add: no room for a plan");
+    const int units = rows / AD_UNIT + (slots < rows ? slots : rows), ranks = rank * slices;
+    int* n_units = (int*)scratch;
+    int4* list = (int4*)scratch + 1;
+    int* order = (int*)(list + units);
+    float* v = (float*)((int4*)scratch + 1 + units + (rows + 3) / 4);
+    adapter_plan_kernel<<<1, 1024, (size_t)slots * 8, s>>>(ids, rows, slots, list, order, n_units);
+    const int rt = ranks <= 16 ? 1 : ranks <= 32 ? 2 : 4;
+    const int part_k = ((K + parts - 1) / parts + 255) / 256 * 256;
+    const dim3 down(units, (K + part_k - 1) / part_k, (ranks + 16 * rt - 1) / (16 * rt));
+    const int cols = 512;
+    const dim3 up(units, (N + cols - 1) / cols);
+    const bool yvec = N % 4 == 0;
+    if (dt == TP_BF16) {
+      if (vec) adapter_down<bf16_t, true>(g, down, rt, list, order, n_units, v, part_k, s);
+      else adapter_down<bf16_t, false>(g, down, rt, list, order, n_units, v, part_k, s);
+      if (yvec) adapter_up_kernel<bf16_t, true><<<up, 256, 0, s>>>(g, list, order, n_units, v, down.y, cols);
+      else adapter_up_kernel<bf16_t, false><<<up, 256, 0, s>>>(g, list, order, n_units, v, down.y, cols);
+    } else {
+      if (vec) adapter_down<float, true>(g, down, rt, list, order, n_units, v, part_k, s);
+      else adapter_down<float, false>(g, down, rt, list, order, n_units, v, part_k, s);
+      if (yvec) adapter_up_kernel<float, true><<<up, 256, 0, s>>>(g, list, order, n_units, v, down.y, cols);
+      else adapter_up_kernel<float, false><<<up, 256, 0, s>>>(g, list, order, n_units, v, down.y, cols);
+    }
+    TP_CHECK_LAUNCH("adapter_add");
+    return 0;
+  }
   const int cols = 256;
+  TP_REQUIRE(rows <= 65535, "adapter_add: too many rows");
   const dim3 grid((N + cols - 1) / cols, rows);
   const size_t lds = (size_t)slices * rank * sizeof(float);
   TP_REQUIRE(lds <= 65536, "adapter_add: ranks of all slices beyond 16,384");

@@ -894,6 +894,10 @@ def linear(x, w: torch.Tensor, out_dtype: torch.dtype, residual: Optional[torch.
 ADAPTER_SLICES = 8
 
 
+#: steps of up to this many rows have a block a row and 256 columns work out its low-rank values for itself (of single tokens four times as many)
+adapter_single_rows = 32
+
+
 class Adapters:
     """Low-rank adapters of one projection of ``n`` columns and ``k`` inputs, one in each slot: ``a`` [slots, slices * rank, k],
     ``b`` [slots, n, rank] (both of the activations' type), ``scales`` float32 [slots].  A projection that several matrices were
@@ -950,8 +954,14 @@ def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, re
     if m == 0:
         return y
     vec = int(k % 8 == 0 and x.data_ptr() % 16 == 0 and adapters.a.data_ptr() % 16 == 0)
+    parts, scratch = 0, None
+    if (m > adapter_single_rows if max_run != 1 else m > 4 * adapter_single_rows) and adapters.slots <= 4096:
+        ranks = adapters.slices * adapters.rank
+        units = m // 64 + min(adapters.slots, m)
+        parts = max(1, min(8, k // 512, 512 // (max(1, m // 64) * -(-ranks // 64))))
+        scratch = torch.empty((4 + 4 * units + -(-m // 4) * 4 + parts * m * ranks,), dtype=torch.float32, device=x.device)
     _call("tp_adapter_add", _ptr(ids), _ptr(x), _dt(x), _ptr(adapters.a), _ptr(adapters.b), _ptr(adapters.scales), _ptr(y), m, k, adapters.n,
-          adapters.slots, adapters.rank, adapters.slices, int(adapters.interleaved), adapters.ends, vec, _stream(), tag=(m, adapters.n, k))
+          adapters.slots, adapters.rank, adapters.slices, int(adapters.interleaved), adapters.ends, vec, parts, _ptr(scratch), _stream(), tag=(m, adapters.n, k))
     return y
 
 

@@ -67,7 +67,9 @@ PORTIONS = [3] * 40 + [-1] * 30 + [0] * 17 + [2] + [3] + [1] * 90
 @pytest.mark.parametrize("k,n,rank", [(512, 320, 16), (264, 1000, 8), (100, 37, 3), (1024, 48, 40), (129, 256, 12)])
 def test_rows(dtype, ids, k, n, rank):
     """One row to many, rows without an adapter, adapters that several requests share; widths and ranks of every alignment."""
-    _check(_case(ids, k, n, rank, 4, dtype=dtype, seed=k + len(ids)))
+    case = _case(ids, k, n, rank, 4, dtype=dtype, seed=k + len(ids))
+    _check(case)
+    _check(case, max_run=1)
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -75,7 +77,8 @@ def test_rows(dtype, ids, k, n, rank):
 @pytest.mark.parametrize("ends,interleaved", [([64, 80, 96], False), ([100, 101, 400], False), ([17, 300], False), ([320], True), ([1, 2, 3, 4, 5, 6, 7, 333], False)])
 def test_slices(dtype, ids, ends, interleaved):
     """Stacked projections: slices that end inside a tile, narrow ones, and two that alternate by eights."""
-    _check(_case(ids, 256, ends[-1], 16, 4, None if interleaved else ends, dtype, seed=len(ends), interleaved=interleaved))
+    for rank in (16, 72):
+        _check(_case(ids, 256, ends[-1], rank, 4, None if interleaved else ends, dtype, seed=len(ends), interleaved=interleaved))
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
@@ -139,3 +142,10 @@ def test_refusals():
                                   (t["a"].cpu(), t["b"], t["scales"], None, False)):
         with pytest.raises(KernelError):
             ops.Adapters(a, b, sc, ends, inter)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_many_adapters_and_long_rows(dtype):
+    """More adapters than one pass of the plan takes, most of them with one row; one adapter with rows all over the batch; K in several parts."""
+    _check(_case([(i * 37) % 1300 - 1 for i in range(400)], 64, 48, 8, 1299, dtype=dtype))
+    _check(_case([0 if i % 3 else (i // 3) % 4 for i in range(700)], 4104, 80, 16, 4, dtype=dtype))
