@@ -32,7 +32,6 @@ typedef unsigned int pa_u32x4 __attribute__((ext_vector_type(4)));
 
 #define PA_WAVES 4
 #define PA_MAX_PARTS 64     // a row's parts: the joining kernel holds one part's statistics a lane
-#define PA_GPTR(p) ((const __attribute__((address_space(1))) void*)(p))
 #define PA_LPTR(p) ((__attribute__((address_space(3))) void*)(p))
 #define PA_WAIT_VM(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
 #define PA_WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
@@ -68,6 +67,7 @@ __device__ inline pa_u32x4 pa_lds(unsigned addr) {
   asm volatile("ds_read_b128 %0, %1" : "=v"(v) : "v"(addr));
   return v;
 }
+__device__ inline void pa_lds_at(unsigned addr, int offset, pa_u32x4& v) { asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(v) : "v"(addr), "n"(offset)); }
 // the maximum over the four lanes of a column
 __device__ inline float pa_column_max(float v) {
   LanePair p = lanes_32(v);
@@ -84,60 +84,231 @@ struct PartRows {
   int part;
 };
 
-// E: bytes of an element.  NB: steps of a wave's ring.  NT: keys and values are read by one block only.
-template <int E, int D, int NQ, int NB, bool NT>
-__device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, const PartRows& w, int kvh) {
-  constexpr int CH = D * E / 16;                              // 16-byte chunks of a key
-  constexpr int SH = CH >= 16 ? 0 : CH == 8 ? 1 : 2;
-  constexpr int KF = CH / 4;                                  // a lane's chunks of a key (or of a row of q)
-  constexpr int DT = D / 16;
-  constexpr int VF = E / 2;                                   // a lane's chunks of an element's 32 keys
-  constexpr int KI = D * E / 32, VI = KI, STAGE = (KI + VI) * 1024;
-  constexpr int VD = 64 / E;                                  // elements of a kilobyte of values (of half a step's keys): 32 or 16
-  static_assert(E == 2 || E == 4, "element size");
-  static_assert((NB == 1 || NB == 2) && 2 * VI + KI <= 63, "the waits below");
-  static_assert(NB * STAGE >= (D * 17 + 32) * 4, "room for the sums of a tile");
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int g = lane >> 4, c = lane & 15;
-  const int group = a.n_heads / a.n_kv;
-  const int psh = a.page_shift, ps = 1 << psh, pmask = ps - 1;
+// Where a lane stands in a step of 32 keys (E: bytes of an element): its place in each kilobyte that is loaded, and its fragments' places in LDS.
+// In LDS a step is its keys as 32 rows of D elements, chunk x of 16 bytes of the row with place i in its tile at (x + f(i)) mod the chunks,
+// so that the 16 rows a quarter of a wave reads fall into different banks; behind them its values in kilobytes of VD elements and half of the keys,
+// the e-th 16 bytes of an element at place VD e + d % VD.
+template <int E, int D>
+struct PrefixLane {
+  static constexpr int CH = D * E / 16, SH = CH >= 16 ? 0 : CH == 8 ? 1 : 2;      // 16-byte chunks of a key
+  static constexpr int KF = CH / 4, DT = D / 16, VF = E / 2;                      // a lane's chunks: of a key, tiles of elements, of an element's 32 keys
+  static constexpr int KI = D * E / 32, STAGE = 2 * KI * 1024, VD = 64 / E;       // loads of a step's keys (values likewise), its bytes
+  unsigned kaddr[2], vaddr;
+  int c, g;
+  __device__ inline PrefixLane(int lane) : c(lane & 15), g(lane >> 4) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) kaddr[t] = (E == 2 ? 8 * (c >> 2) + 4 * t + (c & 3) : 16 * t + c) * (CH * 16);
+    // (bfloat16: the keys 8 g .. lie in half g / 2, chunk g % 2; float32: the keys 16 t + 4 g .. in half t, chunk g)
+    vaddr = KI * 1024 + (E == 2 ? (g >> 1) * 1024 + (g & 1) * 512 : g * 256) + c * 16;
+  }
+  // of load t of the keys: its offset from the first key of its half; of the values: from the half's first place of the load's first element
+  static __device__ inline unsigned key_offset(int t, int lane) {
+    const int row = (64 * t + lane) / CH, pc = (64 * t + lane) % CH;
+    const int i = E == 2 ? 4 * (row >> 3) + (row & 3) : row & 15;
+    return (unsigned)((row & 15) * (D * E) + ((pc - (i >> SH) + CH) % CH) * 16);
+  }
+  static __device__ inline unsigned value_offset(int lane, int ps) { return (unsigned)((lane % VD) * (ps * E) + (lane / VD) * 16); }
+  __device__ inline void read_keys(unsigned base, pa_u32x4 (&kk)[2][KF]) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int f = 0; f < KF; ++f) kk[t][f] = pa_lds(base + kaddr[t] + ((f * 4 + g + (c >> SH)) % CH) * 16);
+  }
+  __device__ inline void read_values(unsigned base, pa_u32x4 (&vv)[DT][VF]) const {
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int t = 0; t < VF; ++t) {
+        const unsigned at = base + vaddr;
+        pa_lds_at(at, (E == 2 ? (dt >> 1) * 2048 + (dt & 1) * 256 : dt * 2048 + t * 1024), vv[dt][t]);
+      }
+  }
+  template <int A, int B>
+  static __device__ inline void arrived(pa_u32x4 (&v)[A][B]) {
+    PA_WAIT_LDS();
+#pragma unroll
+    for (int i = 0; i < A; ++i)
+#pragma unroll
+      for (int j = 0; j < B; ++j) asm volatile("" : "+v"(v[i][j]));
+  }
+};
 
-  // q: this lane's rows of the tiles, and the last key each of them sees
-  pa_u32x4 qf[NQ][KF];
-  int limit[NQ];
+// 16 bytes a lane from base + the lane's offset into a kilobyte of LDS.  (As buffer loads from a uniform base: no vector arithmetic a load.)
+template <bool NT>
+__device__ inline void prefix_copy(const unsigned char* base, unsigned offset, unsigned char* lds) {
+  const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, PA_LPTR(lds), 16, offset, 0, 0, NT ? 2 : 0);
+}
+
+// One step's scores: S^T of both key tiles.
+template <int E, int NQ, int KF>
+__device__ inline void prefix_scores(const pa_u32x4 (&kk)[2][KF], const pa_u32x4 (&qf)[NQ][KF], pa_f32x4 (&s)[NQ][2]) {
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) s[nq][t] = (pa_f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int f = 0; f < KF; ++f)
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (E == 2) {
+          s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, kk[t][f]), __builtin_bit_cast(pa_bf16x8, qf[nq][f]),
+                                                             s[nq][t], 0, 0, 0);
+        } else {
+          const pa_f32x4 kv = __builtin_bit_cast(pa_f32x4, kk[t][f]), qv = __builtin_bit_cast(pa_f32x4, qf[nq][f]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[e], qv[e], s[nq][t], 0, 0, 0);
+        }
+      }
+}
+
+// Scores under a cap: cap * tanh(x) with tanh(x) = 1 - 2 / (2^(2 x log2 e) + 1), in units of log 2; both limits come out right (2^large is
+// infinite, its reciprocal 0).
+template <int NQ>
+__device__ inline void prefix_cap(const PrefixArgs& a, pa_f32x4 (&s)[NQ][2]) {
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        s[nq][t][r] = fmaf(-2.0f * a.cap_log2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[nq][t][r] * a.cap_in) + 1.0f), a.cap_log2);
+}
+
+// Keys outside the part or above the row's limit are not in the sums.
+template <int E, int NQ>
+__device__ inline void prefix_mask(const PartRows& w, int j0, int g, const int (&limit)[NQ], pa_f32x4 (&s)[NQ][2]) {
 #pragma unroll
   for (int nq = 0; nq < NQ; ++nq) {
-    const int pair = w.row0 + min(nq * 16 + c, w.rows - 1);
-    const int token = pair / group, head = kvh * group + pair % group;
-    const unsigned char* row = (const unsigned char*)a.q + ((size_t)(w.token0 + token) * a.n_heads + head) * (D * E) + g * 16;
+    const int hi = min(w.end - 1, limit[nq]);
 #pragma unroll
-    for (int i = 0; i < KF; ++i) qf[nq][i] = *(const pa_u32x4*)(row + i * 64);
+    for (int j = 0; j < 8; ++j) {
+      const int key = j0 + (E == 2 ? 8 * g + j : 16 * (j >> 2) + 4 * g + (j & 3));
+      if (key < w.first || key > hi) s[nq][j >> 2][j & 3] = -INFINITY;
+    }
+  }
+}
+
+// The scores' probabilities, as the next product's operand (pf).  The exponent is one fused multiply-add of the score; the sums so far (l, o) are
+// scaled only when a maximum moved, which is asked once for all tiles, so that one tile's exponentials run beside another's.
+template <int E, int NQ, int DT>
+__device__ inline void prefix_softmax(float scale, pa_f32x4 (&s)[NQ][2], float (&m)[NQ], float (&l)[NQ], pa_u32x4 (&pf)[NQ][E / 2], pa_f32x4 (&o)[NQ][DT]) {
+  float m_new[NQ];
+  bool any = false;
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq) {
+    float top = fmaxf(fmaxf(fmaxf(s[nq][0][0], s[nq][0][1]), fmaxf(s[nq][0][2], s[nq][0][3])),
+                      fmaxf(fmaxf(s[nq][1][0], s[nq][1][1]), fmaxf(s[nq][1][2], s[nq][1][3])));
+    top = pa_column_max(top);
+    m_new[nq] = fmaxf(m[nq], top * scale);     // (the scale is positive)
+    any |= m_new[nq] != m[nq];
+  }
+  if (__builtin_amdgcn_ballot_w64(any) != 0) {
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+      const float shrink = __builtin_amdgcn_exp2f(m[nq] - (m_new[nq] == -INFINITY ? 0.f : m_new[nq]));
+      l[nq] *= shrink;
+      m[nq] = m_new[nq];
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[nq][dt][r] *= shrink;
+    }
+  }
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq) {
+    const float use = m[nq] == -INFINITY ? 0.f : m[nq];   // (a row that has seen no key yet)
+    pa_f32x4 v[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[t][r] = __builtin_amdgcn_exp2f(fmaf(s[nq][t][r], scale, -use));
+    // (this lane's keys; the lanes of a column are added at the end)
+    l[nq] += ((v[0][0] + v[0][1]) + (v[0][2] + v[0][3])) + ((v[1][0] + v[1][1]) + (v[1][2] + v[1][3]));
+    if constexpr (E == 2) {
+      pf[nq][0] = (pa_u32x4){pa_pack(v[0][0], v[0][1]), pa_pack(v[0][2], v[0][3]), pa_pack(v[1][0], v[1][1]), pa_pack(v[1][2], v[1][3])};
+    } else {
+      pf[nq][0] = __builtin_bit_cast(pa_u32x4, v[0]);
+      pf[nq][1] = __builtin_bit_cast(pa_u32x4, v[1]);
+    }
+  }
+}
+
+// Places behind the part's last key hold whatever an earlier owner of the page left there; their probabilities are 0, but 0 * NaN and 0 * Inf are
+// not, so they are cleared.
+template <int E, int DT, int VF>
+__device__ inline void prefix_clear(int end, int j0, int g, pa_u32x4 (&vv)[DT][VF]) {
+#pragma unroll
+  for (int t = 0; t < VF; ++t) {
+    const int left = end - (j0 + (E == 2 ? 8 * g : 16 * t + 4 * g));
+    pa_u32x4 keep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      keep[e] = E == 2 ? (2 * e < left ? 0x0000ffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u) : e < left ? 0xffffffffu : 0u;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) vv[dt][t] &= keep;
+  }
+}
+
+// o += values x probabilities
+template <int E, int NQ, int DT, int VF>
+__device__ inline void prefix_values(const pa_u32x4 (&vv)[DT][VF], const pa_u32x4 (&pf)[NQ][VF], pa_f32x4 (&o)[NQ][DT]) {
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) {
+      if constexpr (E == 2) {
+        o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, vv[dt][0]), __builtin_bit_cast(pa_bf16x8, pf[nq][0]),
+                                                            o[nq][dt], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const pa_f32x4 vv4 = __builtin_bit_cast(pa_f32x4, vv[dt][t]), p4 = __builtin_bit_cast(pa_f32x4, pf[nq][t]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv4[e], p4[e], o[nq][dt], 0, 0, 0);
+        }
+      }
+    }
+}
+
+// q of a wave's rows from `at` of the part's on, their places among all (token, head) rows and the last key each sees.
+template <int E, int D, int NQ, int KF>
+__device__ inline void prefix_queries(const PrefixArgs& a, const PartRows& w, int kvh, int at, int c, int g, pa_u32x4 (&qf)[NQ][KF], int (&limit)[NQ],
+                                      size_t (&row)[NQ]) {
+  const int group = a.n_heads / a.n_kv;
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq) {
+    const int pair = w.row0 + min(at + nq * 16 + c, w.rows - 1), token = pair / group;
+    row[nq] = (size_t)(w.token0 + token) * a.n_heads + kvh * group + pair % group;
+    const unsigned char* q = (const unsigned char*)a.q + row[nq] * (D * E) + g * 16;
+#pragma unroll
+    for (int i = 0; i < KF; ++i) qf[nq][i] = *(const pa_u32x4*)(q + i * 64);
     limit[nq] = w.limit0 == 0x7fffffff ? w.limit0 : w.limit0 + token;
   }
+}
 
-  // this lane's place in each load of a step: of the keys the row's chunk, of the values the element's chunk
+// Few rows: every wave takes all of them and a run of the part's steps, through a ring of its own of one step, filled again as soon as its
+// fragments are in registers; no barrier until the waves' sums are added.  (Two blocks a CU: eight steps on their way.)  NT: keys and values are read by one block only.
+template <int E, int D, int NQ, bool NT>
+__device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, const PartRows& w, int kvh) {
+  using L = PrefixLane<E, D>;
+  constexpr int KF = L::KF, DT = L::DT, VF = L::VF, KI = L::KI;
+  static_assert(2 * KI <= 63 && L::STAGE >= (D * 17 + 32) * 4, "the waits below; room for the sums of a tile");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const L at(lane);
+  const int g = at.g, c = at.c;
+  const int psh = a.page_shift, ps = 1 << psh, pmask = ps - 1;
   unsigned koff[KI];
 #pragma unroll
-  for (int t = 0; t < KI; ++t) {
-    const int row = (64 * t + lane) / CH, pc = (64 * t + lane) % CH;
-    const int i = E == 2 ? 4 * (row >> 3) + (row & 3) : row & 15;       // its place in its tile
-    koff[t] = (unsigned)((row & 15) * (D * E) + ((pc - (i >> SH) + CH) % CH) * 16);
-  }
-  const unsigned voff = (unsigned)((lane % VD) * (ps * E) + (lane / VD) * 16);
+  for (int t = 0; t < KI; ++t) koff[t] = L::key_offset(t, lane);
+  const unsigned voff = L::value_offset(lane, ps);
   const size_t page_bytes = (size_t)a.n_kv * D * ps * E;
   const unsigned char* kbase = (const unsigned char*)a.k_cache + (size_t)kvh * ps * D * E;
   const unsigned char* vbase = (const unsigned char*)a.v_cache + (size_t)kvh * ps * D * E;
-  unsigned char* ring = stages + wave * (NB * STAGE);
+  unsigned char* ring = stages + wave * L::STAGE;
   const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned char*)ring;
-  unsigned kaddr[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) kaddr[t] = (E == 2 ? 8 * (c >> 2) + 4 * t + (c & 3) : 16 * t + c) * (CH * 16);
-  unsigned kchunk[KF];
-#pragma unroll
-  for (int i = 0; i < KF; ++i) kchunk[i] = ((i * 4 + g + (c >> SH)) % CH) * 16;
-  // (bfloat16: the keys 8 g .. lie in half g / 2, chunk g % 2; float32: the keys 16 t + 4 g .. in half t, chunk g)
-  const unsigned vaddr = KI * 1024 + (E == 2 ? (g >> 1) * 1024 + (g & 1) * 512 : g * 256) + c * 16;
-
   // (block tables through the constant address space: uniform loads from it are scalar loads)
   const __attribute__((address_space(4))) int* table = (const __attribute__((address_space(4))) int*)(uintptr_t)w.table;
   const int base16 = w.first & ~15;                           // (a step's halves of 16 keys lie in one page each)
@@ -150,32 +321,23 @@ __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, c
     pp0 = table[j0 >> psh];
     pp1 = table[min(j0 + 16, last16) >> psh];
   };
-  auto issue_keys = [&](int i, int st) __attribute__((always_inline)) {
-    const int j0 = base16 + (w0 + i) * 32;
-    const unsigned char* half[2] = {kbase + (size_t)(unsigned)pp0 * page_bytes + (size_t)(j0 & pmask) * (D * E),
-                                    kbase + (size_t)(unsigned)pp1 * page_bytes + (size_t)(min(j0 + 16, last16) & pmask) * (D * E)};
+  auto issue_keys = [&](int i) __attribute__((always_inline)) {
+    const int j0 = base16 + (w0 + i) * 32, j1 = min(j0 + 16, last16);
+    const unsigned char* b0 = kbase + (size_t)(unsigned)pp0 * page_bytes + (unsigned)((j0 & pmask) * (D * E));
+    const unsigned char* b1 = kbase + (size_t)(unsigned)pp1 * page_bytes + (unsigned)((j1 & pmask) * (D * E));
 #pragma unroll
-    for (int t = 0; t < KI; ++t)
-      __builtin_amdgcn_global_load_lds(PA_GPTR(half[t >= KI / 2] + koff[t]), PA_LPTR(ring + st * STAGE + t * 1024), 16, 0, NT ? 2 : 0);
+    for (int t = 0; t < KI; ++t) prefix_copy<NT>(t >= KI / 2 ? b1 : b0, koff[t], ring + t * 1024);
   };
-  auto issue_values = [&](int i, int st) __attribute__((always_inline)) {
-    const int j0 = base16 + (w0 + i) * 32;
-    const unsigned char* half[2] = {vbase + (size_t)(unsigned)pp0 * page_bytes + (j0 & pmask) * E,
-                                    vbase + (size_t)(unsigned)pp1 * page_bytes + (min(j0 + 16, last16) & pmask) * E};
+  auto issue_values = [&](int i) __attribute__((always_inline)) {
+    const int j0 = base16 + (w0 + i) * 32, j1 = min(j0 + 16, last16);
+    const unsigned char* b0 = vbase + (size_t)(unsigned)pp0 * page_bytes + (unsigned)((j0 & pmask) * E);
+    const unsigned char* b1 = vbase + (size_t)(unsigned)pp1 * page_bytes + (unsigned)((j1 & pmask) * E);
 #pragma unroll
-    for (int t = 0; t < VI; ++t)
-      __builtin_amdgcn_global_load_lds(PA_GPTR(half[t & 1] + (size_t)(t >> 1) * VD * ps * E + voff), PA_LPTR(ring + st * STAGE + (KI + t) * 1024), 16, 0,
-                                       NT ? 2 : 0);
+    for (int t = 0; t < KI; ++t) prefix_copy<NT>(((t & 1) ? b1 : b0) + (size_t)((t >> 1) * L::VD * E) * ps, voff, ring + (KI + t) * 1024);
   };
-#pragma unroll
-  for (int i = 0; i < NB; ++i)
-    if (i < n) {
-      pages_of(i);
-      issue_keys(i, i);
-      issue_values(i, i);
-    }
-  if (NB < n) pages_of(NB);
-
+  pa_u32x4 qf[NQ][KF];
+  int limit[NQ];
+  size_t row[NQ];
   float m[NQ], l[NQ];
   pa_f32x4 o[NQ][DT];
 #pragma unroll
@@ -185,169 +347,64 @@ __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, c
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[nq][dt] = (pa_f32x4){0.f, 0.f, 0.f, 0.f};
   }
-  int st = 0;
-  for (int i = 0; i < n; ++i) {
-    const unsigned base = lds0 + st * STAGE;
-    const bool behind = NB > 1 && i + 1 < n;      // (a whole step on its way behind this one)
-    const bool more = i + NB < n;
-    if (behind) PA_WAIT_VM(VI + KI + VI);
-    else PA_WAIT_VM(VI);
-    const int j0 = base16 + (w0 + i) * 32;
-    pa_u32x4 kk[2][KF];
+  if (n > 0) {
+    pages_of(0);
+    prefix_queries<E, D, NQ, KF>(a, w, kvh, 0, c, g, qf, limit, row);
+    issue_keys(0);
+    issue_values(0);
+    if (n > 1) pages_of(1);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int nq = 0; nq < NQ; ++nq)      // (q is waited for here, in front of the loop, whose waits would else wait for everything)
 #pragma unroll
-      for (int f = 0; f < KF; ++f) kk[t][f] = pa_lds(base + kaddr[t] + kchunk[f]);
-    PA_WAIT_LDS();
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int f = 0; f < KF; ++f) asm volatile("" : "+v"(kk[t][f]));
-    if (more) issue_keys(i + NB, st);
-    pa_f32x4 s[NQ][2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int nq = 0; nq < NQ; ++nq) {
-        s[nq][t] = (pa_f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int f = 0; f < KF; ++f) {
-          if constexpr (E == 2) {
-            s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, kk[t][f]), __builtin_bit_cast(pa_bf16x8, qf[nq][f]),
-                                                               s[nq][t], 0, 0, 0);
-          } else {
-            const pa_f32x4 kv = __builtin_bit_cast(pa_f32x4, kk[t][f]), qv = __builtin_bit_cast(pa_f32x4, qf[nq][f]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[nq][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[e], qv[e], s[nq][t], 0, 0, 0);
-          }
-        }
+      for (int i = 0; i < KF; ++i) asm volatile("" : "+v"(qf[nq][i]));
+    float cap = a.cap_in;
+    const float scale = cap > 0.f ? 1.f : a.scale_log2;
+    for (int i = 0; i < n; ++i) {
+      asm volatile("" : "+s"(cap));      // (a branch of a few instructions, not two loops)
+      const bool more = i + 1 < n;
+      const int j0 = base16 + (w0 + i) * 32;
+      PA_WAIT_VM(KI);
+      pa_u32x4 kk[2][KF], vv[DT][VF];
+      at.read_keys(lds0, kk);
+      L::arrived(kk);
+      if (more) issue_keys(i + 1);
+      pa_f32x4 sc[NQ][2];
+      pa_u32x4 pf[NQ][VF];
+      prefix_scores<E, NQ, KF>(kk, qf, sc);
+      if (cap > 0.f) prefix_cap<NQ>(a, sc);
+      if (j0 < w.first || j0 + 32 > w.end || w.limit0 < j0 + 31) prefix_mask<E, NQ>(w, j0, g, limit, sc);
+      prefix_softmax<E, NQ, DT>(scale, sc, m, l, pf, o);
+      if (more) PA_WAIT_VM(KI);
+      else PA_WAIT_VM(0);
+      at.read_values(lds0, vv);
+      L::arrived(vv);
+      if (more) {
+        issue_values(i + 1);
+        if (i + 2 < n) pages_of(i + 2);
       }
-    // (scores outside the part or above the row's limit: not in the sums; `whole`: none of this step's)
-    const bool whole = j0 >= w.first && j0 + 32 <= w.end && w.limit0 >= j0 + 31;
-    pa_u32x4 pf[NQ][E == 2 ? 1 : 2];
-    float alpha[NQ];
-    bool moved[NQ];
-#pragma unroll
-    for (int nq = 0; nq < NQ; ++nq) {
-      float v[8], top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = s[nq][j >> 2][j & 3] * a.scale_log2;
-      if (a.cap_in > 0.f) {
-        // cap * tanh(x) with tanh(x) = 1 - 2 / (2^(2 x log2 e) + 1); both limits come out right (2^large is infinite, its reciprocal 0)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          v[j] = fmaf(-2.0f * a.cap_log2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[nq][j >> 2][j & 3] * a.cap_in) + 1.0f), a.cap_log2);
-      }
-      if (!whole) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = j0 + (E == 2 ? 8 * g + j : 16 * (j >> 2) + 4 * g + (j & 3));
-          if (key < w.first || key >= w.end || key > limit[nq]) v[j] = -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = fmaxf(top, v[j]);
-      const float m_new = fmaxf(m[nq], pa_column_max(top));
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;   // (a row that has seen no key yet)
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] = __builtin_amdgcn_exp2f(v[j] - m_use);
-        sum += v[j];
-      }
-      moved[nq] = __builtin_amdgcn_ballot_w64(m_new != m[nq]) != 0;
-      alpha[nq] = 1.f;
-      if (moved[nq]) {
-        alpha[nq] = __builtin_amdgcn_exp2f(m[nq] - m_use);
-        m[nq] = m_new;
-      }
-      l[nq] = fmaf(l[nq], alpha[nq], sum);     // (this lane's keys; the lanes of a column are added at the end)
-      if constexpr (E == 2) {
-        pf[nq][0] = (pa_u32x4){pa_pack(v[0], v[1]), pa_pack(v[2], v[3]), pa_pack(v[4], v[5]), pa_pack(v[6], v[7])};
-      } else {
-        pf[nq][0] = __builtin_bit_cast(pa_u32x4, (pa_f32x4){v[0], v[1], v[2], v[3]});
-        pf[nq][1] = __builtin_bit_cast(pa_u32x4, (pa_f32x4){v[4], v[5], v[6], v[7]});
-      }
+      if (j0 + 32 > w.end) prefix_clear<E, DT, VF>(w.end, j0, g, vv);
+      prefix_values<E, NQ, DT, VF>(vv, pf, o);
     }
-    if (more && behind) PA_WAIT_VM(KI + KI + VI);
-    else if (more) PA_WAIT_VM(KI);
-    else if (behind) PA_WAIT_VM(KI + VI);
-    else PA_WAIT_VM(0);
-    pa_u32x4 vv[DT][VF];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int t = 0; t < VF; ++t)
-        vv[dt][t] = pa_lds(base + vaddr + (E == 2 ? (dt >> 1) * 2048 + (dt & 1) * 256 : dt * 2048 + t * 1024));
-    PA_WAIT_LDS();
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int t = 0; t < VF; ++t) asm volatile("" : "+v"(vv[dt][t]));
-    if (more) {
-      issue_values(i + NB, st);
-      if (i + NB + 1 < n) pages_of(i + NB + 1);
-    }
-    if (j0 + 32 > w.end) {
-      // places behind the last key hold whatever an earlier owner of the page left there; their probabilities are 0, but 0 * NaN
-      // and 0 * Inf are not, so they are cleared
-#pragma unroll
-      for (int t = 0; t < VF; ++t) {
-        const int left = w.end - (j0 + (E == 2 ? 8 * g : 16 * t + 4 * g));
-        pa_u32x4 keep;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          keep[e] = E == 2 ? (2 * e < left ? 0x0000ffffu : 0u) | (2 * e + 1 < left ? 0xffff0000u : 0u) : e < left ? 0xffffffffu : 0u;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) vv[dt][t] &= keep;
-      }
-    }
-#pragma unroll
-    for (int nq = 0; nq < NQ; ++nq) {
-      if (moved[nq]) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[nq][dt][r] *= alpha[nq];
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        if constexpr (E == 2) {
-          o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, vv[dt][0]), __builtin_bit_cast(pa_bf16x8, pf[nq][0]),
-                                                              o[nq][dt], 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const pa_f32x4 vv4 = __builtin_bit_cast(pa_f32x4, vv[dt][t]), p4 = __builtin_bit_cast(pa_f32x4, pf[nq][t]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv4[e], p4[e], o[nq][dt], 0, 0, 0);
-          }
-        }
-      }
-    }
-    st = st + 1 == NB ? 0 : st + 1;
   }
 
   // The waves' sums, added in their order through LDS, a tile of 16 rows at a time (rows a bank apart: 17 floats an element)
+  const int group = a.n_heads / a.n_kv;
   float* red = (float*)stages;
   float* stat = red + PA_WAVES * D * 17;
+#pragma unroll
   for (int nq = 0; nq < NQ; ++nq) {
     __syncthreads();     // (every ring is empty; the tile before is read)
+    float sum = l[nq];
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (g == 0) {
+      stat[wave * 32 + c] = m[nq];
+      stat[wave * 32 + 16 + c] = sum;
+    }
 #pragma unroll
-    for (int k = 0; k < NQ; ++k)
-      if (k == nq) {     // (constant places: the sums stay in registers)
-        float sum = l[k];
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (g == 0) {
-          stat[wave * 32 + c] = m[k];
-          stat[wave * 32 + 16 + c] = sum;
-        }
+    for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) red[(wave * D + dt * 16 + 4 * g + r) * 17 + c] = o[k][dt][r];
-      }
+      for (int r = 0; r < 4; ++r) red[(wave * D + dt * 16 + 4 * g + r) * 17 + c] = o[nq][dt][r];
     __syncthreads();
     const int rows = min(16, w.rows - nq * 16);
     for (int e = threadIdx.x; e < D * rows; e += PA_WAVES * 64) {
@@ -356,25 +413,138 @@ __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, c
 #pragma unroll
       for (int v = 1; v < PA_WAVES; ++v) top = fmaxf(top, stat[v * 32 + col]);
       const float use = top == -INFINITY ? 0.f : top;
-      float acc = 0.f, sum = 0.f;
+      float acc = 0.f, total = 0.f;
 #pragma unroll
       for (int v = 0; v < PA_WAVES; ++v) {
         const float f = __builtin_amdgcn_exp2f(stat[v * 32 + col] - use);
         acc = fmaf(f, red[(v * D + d) * 17 + col], acc);
-        sum = fmaf(f, stat[v * 32 + 16 + col], sum);
+        total = fmaf(f, stat[v * 32 + 16 + col], total);
       }
       const int pair = w.row0 + nq * 16 + col;
-      const size_t at = ((size_t)(w.token0 + pair / group) * a.n_heads + kvh * group + pair % group) * a.parts + w.part;
-      a.sums[at * D + d] = acc;
-      if (d == 0) *(float2*)(a.stats + at * 2) = make_float2(top, sum);
+      const size_t to = ((size_t)(w.token0 + pair / group) * a.n_heads + kvh * group + pair % group) * a.parts + w.part;
+      a.sums[to * D + d] = acc;
+      if (d == 0) *(float2*)(a.stats + to * 2) = make_float2(top, total);
     }
   }
 }
 
-// NQS, NQO: tiles of 16 rows of a block with shared and with own keys.
-template <int E, int D, int NQS, int NQO, int NB, int OCC>
+// Many rows: the four waves take 16 * NQ rows each and walk the part's steps together, through a ring of NS steps that all of them fill, a quarter each,
+// NS - 1 steps ahead; one barrier a step.  So a CU loads a step once for 64 * NQ rows, and one wave's products run beside another's exponentials.
+template <int E, int D, int NQ, int NS>
+__device__ inline void prefix_part_rows(const PrefixArgs& a, unsigned char* stages, const PartRows& w, int kvh) {
+  using L = PrefixLane<E, D>;
+  constexpr int KF = L::KF, DT = L::DT, VF = L::VF, KI = L::KI;
+  constexpr int LOADS = 2 * KI / PA_WAVES;
+  static_assert(NS >= 2 && (2 * KI) % PA_WAVES == 0 && (NS - 1) * LOADS <= 63, "a quarter of a step's loads");
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const L at(lane);
+  const int g = at.g, c = at.c;
+  const int psh = a.page_shift, ps = 1 << psh, pmask = ps - 1;
+  const size_t page_bytes = (size_t)a.n_kv * D * ps * E;
+  const unsigned char* kbase = (const unsigned char*)a.k_cache + (size_t)kvh * ps * D * E;
+  const unsigned char* vbase = (const unsigned char*)a.v_cache + (size_t)kvh * ps * D * E;
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) const unsigned char*)stages;
+  const __attribute__((address_space(4))) int* table = (const __attribute__((address_space(4))) int*)(uintptr_t)w.table;
+  const int base16 = w.first & ~15, n = (w.end - base16 + 31) >> 5, last16 = (w.end - 1) & ~15;
+  // this wave's loads of a step: LOADS of the 2 KI kilobytes, the keys' first.  A wave's loads lie in one half of the keys, and of keys or values alone
+  // (but for the smallest heads: two waves load keys, two values, either way)
+  const int t0 = wave * LOADS;
+  const bool of_keys = t0 < KI;
+  unsigned off[LOADS];
+  int half[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int t = t0 + j;
+    off[j] = of_keys ? L::key_offset(t, lane) : L::value_offset(lane, ps) + (unsigned)(((t - KI) >> 1) * L::VD * E) * ps;
+    half[j] = of_keys ? (t >= KI / 2) : (t - KI) & 1;
+  }
+  int pp0 = 0, pp1 = 0;
+  auto pages_of = [&](int i) {
+    const int j0 = base16 + i * 32;
+    pp0 = table[j0 >> psh];
+    pp1 = table[min(j0 + 16, last16) >> psh];
+  };
+  const unsigned char* mine = of_keys ? kbase : vbase;
+  const int key_bytes = of_keys ? D * E : E;
+  auto issue = [&](int i, int st) __attribute__((always_inline)) {
+    const int j0 = base16 + i * 32, j1 = min(j0 + 16, last16);
+    const unsigned char* b0 = mine + (size_t)(unsigned)pp0 * page_bytes + (unsigned)((j0 & pmask) * key_bytes);
+    const unsigned char* b1 = mine + (size_t)(unsigned)pp1 * page_bytes + (unsigned)((j1 & pmask) * key_bytes);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) prefix_copy<false>(half[j] ? b1 : b0, off[j], stages + st * L::STAGE + (t0 + j) * 1024);
+  };
+  pa_u32x4 qf[NQ][KF];
+  int limit[NQ];
+  size_t row[NQ];
+  float m[NQ], l[NQ];
+  pa_f32x4 o[NQ][DT];
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq) {
+    m[nq] = -INFINITY;
+    l[nq] = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[nq][dt] = (pa_f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  prefix_queries<E, D, NQ, KF>(a, w, kvh, wave * NQ * 16, c, g, qf, limit, row);
+  // (steps that are not there: the last one again, so that the loads on their way are always as many as the waits below count)
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) {
+    pages_of(min(i, n - 1));
+    issue(min(i, n - 1), i);
+  }
+  pages_of(min(NS - 1, n - 1));
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+    for (int i = 0; i < KF; ++i) asm volatile("" : "+v"(qf[nq][i]));
+  const bool busy = wave * NQ * 16 < w.rows;      // (a wave without rows loads for the others)
+  int st = 0;
+  float cap = a.cap_in;
+  const float scale = cap > 0.f ? 1.f : a.scale_log2;
+  for (int i = 0; i < n; ++i) {
+    asm volatile("" : "+s"(cap));        // (a branch of a few instructions, not two loops)
+    PA_WAIT_VM((NS - 2) * LOADS);
+    __builtin_amdgcn_s_barrier();                 // every wave's share of this step has come, and the step before is read by all
+    asm volatile("" ::: "memory");
+    issue(min(i + NS - 1, n - 1), st == 0 ? NS - 1 : st - 1);
+    pages_of(min(i + NS, n - 1));
+    const unsigned base = lds0 + st * L::STAGE;
+    st = st + 1 == NS ? 0 : st + 1;
+    if (!busy) continue;
+    const int j0 = base16 + i * 32;
+    pa_u32x4 kk[2][KF], vv[DT][VF];
+    at.read_keys(base, kk);
+    L::arrived(kk);
+    pa_f32x4 sc[NQ][2];
+    pa_u32x4 pf[NQ][VF];
+    prefix_scores<E, NQ, KF>(kk, qf, sc);
+    at.read_values(base, vv);
+    if (cap > 0.f) prefix_cap<NQ>(a, sc);
+    if (j0 < w.first || j0 + 32 > w.end || w.limit0 < j0 + 31) prefix_mask<E, NQ>(w, j0, g, limit, sc);
+    prefix_softmax<E, NQ, DT>(scale, sc, m, l, pf, o);
+    L::arrived(vv);
+    if (j0 + 32 > w.end) prefix_clear<E, DT, VF>(w.end, j0, g, vv);
+    prefix_values<E, NQ, DT, VF>(vv, pf, o);
+  }
+  PA_WAIT_VM(0);       // (nothing is on its way into LDS when the block ends)
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq) {
+    float sum = l[nq];
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if ((wave * NQ + nq) * 16 + c >= w.rows) continue;
+    const size_t to = row[nq] * a.parts + w.part;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) *(pa_f32x4*)(a.sums + to * D + dt * 16 + 4 * g) = o[nq][dt];
+    if (g == 0) *(float2*)(a.stats + to * 2) = make_float2(m[nq], sum);
+  }
+}
+
+// NQS, NQO: tiles of 16 rows of a block with shared and with own keys; NS > 0: of a wave of a block with shared keys, whose waves share their steps.
+template <int E, int D, int NQS, int NQO, int NS, int OCC>
 __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(PrefixArgs a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char stages[PA_WAVES * NB * D * 64 * E];
+  __shared__ __attribute__((aligned(1024))) unsigned char stages[(NS > PA_WAVES ? NS : PA_WAVES) * PrefixLane<E, D>::STAGE];
+  constexpr int ROWS = 16 * NQS * (NS > 0 ? PA_WAVES : 1);      // of a block with shared keys
   const int kvh = blockIdx.x % a.n_kv, group = a.n_heads / a.n_kv;
   int b = blockIdx.x / a.n_kv;
   PartRows w;
@@ -393,7 +563,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(Pr
         token0 = a.cu_seqlens[r0];
         tokens = a.cu_seqlens[a.group_starts[i + 1]] - token0;
       }
-      const int blocks = keys > 0 ? (tokens * group + 16 * NQS - 1) / (16 * NQS) : 0;
+      const int blocks = keys > 0 ? (tokens * group + ROWS - 1) / ROWS : 0;
       int upto = blocks;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
@@ -403,10 +573,10 @@ __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(Pr
       const unsigned long long hit = __ballot(rb < upto);
       if (hit != 0) {
         const int src = (int)__builtin_ctzll(hit);
-        w.row0 = (rb - __builtin_amdgcn_readlane(upto - blocks, src)) * 16 * NQS;
+        w.row0 = (rb - __builtin_amdgcn_readlane(upto - blocks, src)) * ROWS;
         w.end = __builtin_amdgcn_readlane(keys, src);
         w.token0 = __builtin_amdgcn_readlane(token0, src);
-        w.rows = min(16 * NQS, __builtin_amdgcn_readlane(tokens, src) * group - w.row0);
+        w.rows = min(ROWS, __builtin_amdgcn_readlane(tokens, src) * group - w.row0);
         w.table = a.block_tables + (size_t)__builtin_amdgcn_readlane(r0, src) * a.table_width;
         found = true;
       }
@@ -417,7 +587,8 @@ __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(Pr
     if (w.first >= w.end) return;
     w.end = min(w.end, w.first + a.shared_steps * 32);
     w.limit0 = 0x7fffffff;
-    prefix_part<E, D, NQS, NB, false>(a, stages, w, kvh);
+    if constexpr (NS > 0) prefix_part_rows<E, D, NQS, NS>(a, stages, w, kvh);
+    else prefix_part<E, D, NQS, false>(a, stages, w, kvh);
     return;
   }
   b -= a.shared_blocks;
@@ -433,7 +604,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(Pr
   w.limit0 = ctx - tokens;
   w.table = a.block_tables + (size_t)r * a.table_width;
   w.part = a.shared_parts + part;
-  prefix_part<E, D, NQO, NB, true>(a, stages, w, kvh);
+  prefix_part<E, D, NQO, true>(a, stages, w, kvh);
 }
 
 // out[token, head, :] from a row's parts, in ascending order: those of its request's shared keys, then those of its own.  A wave a row; its lane
@@ -475,40 +646,45 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restric
   }
 }
 
-template <int E, int D, int NQS, int NQO, int NB, int OCC>
-static void prefix_launch(const PrefixArgs& a, int blocks, hipStream_t s) {
-  prefix_attention_kernel<E, D, NQS, NQO, NB, OCC><<<blocks, PA_WAVES * 64, 0, s>>>(a);
+template <int E, int D, int NQS, int NQO, int NS>
+static int prefix_launch(const PrefixArgs& a, int blocks, hipStream_t s) {
+  prefix_attention_kernel<E, D, NQS, NQO, NS, E == 2 ? 2 : 1><<<blocks, PA_WAVES * 64, 0, s>>>(a);
+  return 0;
 }
 
 template <int E, int D>
-static int prefix_sizes(const PrefixArgs& a, int blocks, int tiles_shared, int tiles_own, hipStream_t s) {
-  constexpr int OCC = E == 2 ? 2 : 1;
-  if (tiles_shared == 1 && tiles_own == 1) prefix_launch<E, D, 1, 1, 1, OCC>(a, blocks, s);
-  else if (tiles_shared == 2 && tiles_own == 1) prefix_launch<E, D, 2, 1, 1, OCC>(a, blocks, s);
-  else if (tiles_shared == 2 && tiles_own == 2) prefix_launch<E, D, 2, 2, 1, OCC>(a, blocks, s);
-  else {
-    tp_set_error("prefix_attention: no kernel for %d and %d tiles", tiles_shared, tiles_own);
-    return 1;
+static int prefix_sizes(const PrefixArgs& a, int blocks, int rows_shared, int rows_own, hipStream_t s) {
+  constexpr int NS = E == 2 ? 4 : 2;
+  if (rows_own == 16) {
+    if (rows_shared == 16) return prefix_launch<E, D, 1, 1, 0>(a, blocks, s);
+    if (rows_shared == 32) return prefix_launch<E, D, 2, 1, 0>(a, blocks, s);
+    if (rows_shared == 64) return prefix_launch<E, D, 1, 1, NS>(a, blocks, s);
+    if (rows_shared == 128) return prefix_launch<E, D, 2, 1, NS>(a, blocks, s);
+  } else if (rows_own == 32) {
+    if (rows_shared == 32) return prefix_launch<E, D, 2, 2, 0>(a, blocks, s);
+    if (rows_shared == 64) return prefix_launch<E, D, 1, 2, NS>(a, blocks, s);
+    if (rows_shared == 128) return prefix_launch<E, D, 2, 2, NS>(a, blocks, s);
   }
-  return 0;
+  tp_set_error("prefix_attention: no kernel for blocks of %d and %d rows", rows_shared, rows_own);
+  return 1;
 }
 
 // q [n, heads, dim] over pages of keys and transposed values (elements of dt), each request's context by its block table; out [n, heads * dim].
 // groups of requests share their first keys (group_starts [groups + 1], group_keys [groups], shared_keys [requests]: see PrefixArgs); every query
-// lies behind its request's shared keys.  shared_rows: at least as many blocks of 16 * tiles_shared rows as all groups have.  Parts of
+// lies behind its request's shared keys.  shared_blocks: at least as many blocks of rows_shared rows (16, 32, 64 or 128) as all groups have; rows_own 16 or 32.  Parts of
 // shared_steps / own_steps steps of 32 keys, as many as there are at most.  scratch: n * heads * (shared_parts + own_parts) * (dim + 2) floats.
 extern "C" int tp_prefix_attention(const void* q, int dt, const void* k_cache, const void* v_cache, const int* block_tables, int table_width,
                                    const int* cu_seqlens, const int* context_lens, const int* token_req, const int* group_starts,
                                    const int* group_keys, const int* shared_keys, void* out, float* scratch, int n, int requests, int groups,
                                    int heads, int kv_heads, int dim, int page_size, float scale, float softcap, const float* sink, int max_q_len,
-                                   int tiles_shared, int tiles_own, int shared_rows, int shared_steps, int shared_parts, int own_steps, int own_parts,
+                                   int rows_shared, int rows_own, int shared_blocks, int shared_steps, int shared_parts, int own_steps, int own_parts,
                                    hipStream_t s) {
   if (n <= 0 || requests <= 0) return 0;
   TP_REQUIRE(dt == TP_BF16 || dt == TP_F32, "prefix_attention: unsupported element type");
   TP_REQUIRE(dim == 32 || dim == 64 || dim == 128, "prefix_attention: heads of 32, 64 or 128 elements");
   TP_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "prefix_attention: pages of a power of two from 16 on");
   TP_REQUIRE(kv_heads > 0 && heads % kv_heads == 0 && groups > 0 && max_q_len > 0, "prefix_attention: bad sizes");
-  TP_REQUIRE(shared_steps > 0 && own_steps > 0 && shared_parts > 0 && own_parts > 0 && shared_parts + own_parts <= PA_MAX_PARTS && shared_rows > 0,
+  TP_REQUIRE(shared_steps > 0 && own_steps > 0 && shared_parts > 0 && own_parts > 0 && shared_parts + own_parts <= PA_MAX_PARTS && shared_blocks > 0 && rows_own > 0,
              "prefix_attention: bad parts");
   PrefixArgs a = {};
   a.q = q;
@@ -529,24 +705,24 @@ extern "C" int tp_prefix_attention(const void* q, int dt, const void* k_cache, c
   a.n_kv = kv_heads;
   a.groups = groups;
   a.requests = requests;
-  a.shared_rows = shared_rows;
+  a.shared_rows = shared_blocks;
   a.shared_parts = shared_parts;
-  a.own_rows = (int)(((long)max_q_len * (heads / kv_heads) + 16 * tiles_own - 1) / (16 * tiles_own));
+  a.own_rows = (int)(((long)max_q_len * (heads / kv_heads) + rows_own - 1) / rows_own);
   a.shared_steps = shared_steps;
   a.own_steps = own_steps;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.cap_log2 = softcap * 1.4426950408889634f;
   a.cap_in = softcap > 0.f ? 2.0f * a.scale_log2 / softcap : 0.f;
-  const long shared_blocks = (long)shared_rows * shared_parts, blocks = (shared_blocks + (long)a.own_rows * requests * own_parts) * kv_heads;
+  const long of_shared = (long)shared_blocks * shared_parts, blocks = (of_shared + (long)a.own_rows * requests * own_parts) * kv_heads;
   TP_REQUIRE(blocks < (1L << 31), "prefix_attention: too many blocks");
-  a.shared_blocks = (int)shared_blocks;
+  a.shared_blocks = (int)of_shared;
   int rc = 1;
   if (dt == TP_BF16)
-    rc = dim == 32 ? prefix_sizes<2, 32>(a, (int)blocks, tiles_shared, tiles_own, s) : dim == 64 ? prefix_sizes<2, 64>(a, (int)blocks, tiles_shared, tiles_own, s)
-                                                                                            : prefix_sizes<2, 128>(a, (int)blocks, tiles_shared, tiles_own, s);
+    rc = dim == 32 ? prefix_sizes<2, 32>(a, (int)blocks, rows_shared, rows_own, s) : dim == 64 ? prefix_sizes<2, 64>(a, (int)blocks, rows_shared, rows_own, s)
+                                                                                            : prefix_sizes<2, 128>(a, (int)blocks, rows_shared, rows_own, s);
   else
-    rc = dim == 32 ? prefix_sizes<4, 32>(a, (int)blocks, tiles_shared, tiles_own, s) : dim == 64 ? prefix_sizes<4, 64>(a, (int)blocks, tiles_shared, tiles_own, s)
-                                                                                            : prefix_sizes<4, 128>(a, (int)blocks, tiles_shared, tiles_own, s);
+    rc = dim == 32 ? prefix_sizes<4, 32>(a, (int)blocks, rows_shared, rows_own, s) : dim == 64 ? prefix_sizes<4, 64>(a, (int)blocks, rows_shared, rows_own, s)
+                                                                                            : prefix_sizes<4, 128>(a, (int)blocks, rows_shared, rows_own, s);
   if (rc != 0) return rc;
   TP_CHECK_LAUNCH("prefix_attention");
   const int rows = n * heads, grid = (rows + 3) / 4;

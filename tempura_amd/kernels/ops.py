@@ -1539,17 +1539,23 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if n == 0:
         return out
     group = heads // kvh
-    tiles = 1 if min(n, shared.max_requests * max_q_len) * group <= 16 else 2
-    own_tiles = 1 if max_q_len * group <= 16 else 2
-    rows = n * group // (16 * tiles) + shared.sharing
-    shared_steps, shared_parts = _prefix_parts(-(-shared.max_keys // 32), rows * kvh, 48)
-    own_steps, own_parts = _prefix_parts((own + 15 + 31) // 32, r * -(-max_q_len * group // (16 * own_tiles)) * kvh, 16)
+    rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts = _prefix_plan(n, r, group, kvh, max_q_len, shared, own, q.dtype)
     scratch = torch.empty((n * heads * (shared_parts + own_parts) * (d + 2),), dtype=torch.float32, device=q.device)
     _call("tp_prefix_attention", _ptr(q), _dt(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), width, _ptr(cu_seqlens), _ptr(context_lens),
           _ptr(token_req), _ptr(shared.starts), _ptr(shared.keys), _ptr(shared.each), _ptr(out), _ptr(scratch), n, r, shared.groups, heads, kvh, d,
-          page_size, float(scale), float(softcap), _ptr(sink), int(max_q_len), tiles, own_tiles, rows, shared_steps, shared_parts, own_steps, own_parts,
+          page_size, float(scale), float(softcap), _ptr(sink), int(max_q_len), rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts,
           _stream())
     return out
+
+
+def _prefix_plan(n, r, group, kvh, max_q_len, shared, own, dtype):
+    most = min(n, shared.max_requests * max_q_len) * group
+    rows = 16 if most <= 16 else 32 if most <= 32 else 64 if most <= 64 else 128
+    own_rows = 16 if max_q_len * group <= 16 else 32
+    blocks = n * group // rows + shared.sharing
+    shared_steps, shared_parts = _prefix_parts(-(-shared.max_keys // 32), blocks * kvh, 48)
+    own_steps, own_parts = _prefix_parts((own + 15 + 31) // 32, r * -(-max_q_len * group // own_rows) * kvh, 16)
+    return rows, own_rows, blocks, shared_steps, shared_parts, own_steps, own_parts
 
 
 def _prefix_parts(steps: int, blocks: int, most: int) -> tuple:
