@@ -14,8 +14,8 @@
 // the rows 4 g + r of column c.  bfloat16: the two key tiles of a step take their keys in the order 8 (i / 4) + 4 t + i % 4, so a lane
 // ends up with the eight CONSECUTIVE keys 8 g .. of its row, the operand of the next product.  float32: the order is 16 t + i, a lane has
 // the keys 16 t + 4 g + r, and the product with register r of tile t takes exactly these as its four k.  A fragment is 16 bytes a lane either way.
-// Statistics and sums are float32; the probabilities of bfloat16 caches are rounded to bfloat16 for the second product (the largest
-// is 1, so their errors, up to 2^-9 of each, average out in the sum, which is rounded to bfloat16 anyway).
+// Statistics and sums are float32; the probabilities of bfloat16 caches are rounded to bfloat16 for the second product (errors of up to
+// 2^-8 of each, which average out in the sum, itself rounded to bfloat16 at the end).
 //
 // Each of a block's four waves takes a run of the part's steps and has a ring of NB steps in LDS for itself, filled by direct
 // global-to-LDS loads (whole kilobytes) and emptied without a barrier: a step's keys go on their way as soon as the fragments of the
@@ -31,7 +31,7 @@ typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int pa_u32x4 __attribute__((ext_vector_type(4)));
 
 #define PA_WAVES 4
-#define PA_MAX_PARTS 64     // a row's parts: the joining kernel holds one part's statistics a lane
+#define PA_MAX_PARTS 128    // a row's parts: the joining kernel holds two parts' statistics a lane
 #define PA_LPTR(p) ((__attribute__((address_space(3))) void*)(p))
 #define PA_WAIT_VM(n) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(n) : "memory")
 #define PA_WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory")
@@ -49,6 +49,7 @@ struct PrefixArgs {
   float* sums;               // [token, head, part, D]
   float* stats;              // [token, head, part, 2]: maximum, sum
   int table_width, page_shift, n_heads, n_kv, groups, requests;
+  int single;                // every request brings one token: request r's is token r
   int shared_blocks;         // blocks (of rows and parts) that take shared keys, a key head each; the own keys' come behind them
   int shared_rows;           // blocks of rows among them (an upper bound: those beyond the last group end at once)
   int own_rows;              // blocks of rows of a request
@@ -191,26 +192,28 @@ __device__ inline void prefix_mask(const PartRows& w, int j0, int g, const int (
   }
 }
 
-// The scores' probabilities, as the next product's operand (pf).  The exponent is one fused multiply-add of the score; the sums so far (l, o) are
-// scaled only when a maximum moved, which is asked once for all tiles, so that one tile's exponentials run beside another's.
+// The scores' probabilities, as the next product's operand (pf): 2^(score - m), one fused multiply-add and one exponential each.  m is a maximum seen
+// before, and stays while no score is more than PA_SLACK above it: probabilities up to 2^PA_SLACK are as exact, relative to each other, as those up to 1
+// (float32 sums, bfloat16 roundings), and the sums so far need not be scaled, nor the lanes' maxima compared, in almost any step.  (With a maximum that
+// is one in every step, one of 32 rows moves it in most of the first thirty.)
+#define PA_SLACK 8.0f
 template <int E, int NQ, int DT>
 __device__ inline void prefix_softmax(float scale, pa_f32x4 (&s)[NQ][2], float (&m)[NQ], float (&l)[NQ], pa_u32x4 (&pf)[NQ][E / 2], pa_f32x4 (&o)[NQ][DT]) {
-  float m_new[NQ];
-  bool any = false;
+  float top[NQ];
+  bool above = false;
 #pragma unroll
   for (int nq = 0; nq < NQ; ++nq) {
-    float top = fmaxf(fmaxf(fmaxf(s[nq][0][0], s[nq][0][1]), fmaxf(s[nq][0][2], s[nq][0][3])),
-                      fmaxf(fmaxf(s[nq][1][0], s[nq][1][1]), fmaxf(s[nq][1][2], s[nq][1][3])));
-    top = pa_column_max(top);
-    m_new[nq] = fmaxf(m[nq], top * scale);     // (the scale is positive)
-    any |= m_new[nq] != m[nq];
+    top[nq] = scale * fmaxf(fmaxf(fmaxf(s[nq][0][0], s[nq][0][1]), fmaxf(s[nq][0][2], s[nq][0][3])),     // (the scale is positive)
+                            fmaxf(fmaxf(s[nq][1][0], s[nq][1][1]), fmaxf(s[nq][1][2], s[nq][1][3])));
+    above |= top[nq] > m[nq] + PA_SLACK;
   }
-  if (__builtin_amdgcn_ballot_w64(any) != 0) {
+  if (__builtin_amdgcn_ballot_w64(above) != 0) {
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
-      const float shrink = __builtin_amdgcn_exp2f(m[nq] - (m_new[nq] == -INFINITY ? 0.f : m_new[nq]));
+      const float m_new = fmaxf(m[nq], pa_column_max(top[nq]));
+      const float shrink = __builtin_amdgcn_exp2f(m[nq] - (m_new == -INFINITY ? 0.f : m_new));
       l[nq] *= shrink;
-      m[nq] = m_new[nq];
+      m[nq] = m_new;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -318,8 +321,8 @@ __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, c
   int pp0 = 0, pp1 = 0;
   auto pages_of = [&](int i) {
     const int j0 = base16 + (w0 + i) * 32;
-    pp0 = table[j0 >> psh];
-    pp1 = table[min(j0 + 16, last16) >> psh];
+    pp0 = max(table[j0 >> psh], 0);      // (an entry that names no page reads page 0, not what lies in front of the pool)
+    pp1 = max(table[min(j0 + 16, last16) >> psh], 0);
   };
   auto issue_keys = [&](int i) __attribute__((always_inline)) {
     const int j0 = base16 + (w0 + i) * 32, j1 = min(j0 + 16, last16);
@@ -461,8 +464,8 @@ __device__ inline void prefix_part_rows(const PrefixArgs& a, unsigned char* stag
   int pp0 = 0, pp1 = 0;
   auto pages_of = [&](int i) {
     const int j0 = base16 + i * 32;
-    pp0 = table[j0 >> psh];
-    pp1 = table[min(j0 + 16, last16) >> psh];
+    pp0 = max(table[j0 >> psh], 0);      // (an entry that names no page reads page 0, not what lies in front of the pool)
+    pp1 = max(table[min(j0 + 16, last16) >> psh], 0);
   };
   const unsigned char* mine = of_keys ? kbase : vbase;
   const int key_bytes = of_keys ? D * E : E;
@@ -540,11 +543,20 @@ __device__ inline void prefix_part_rows(const PrefixArgs& a, unsigned char* stag
   }
 }
 
-// NQS, NQO: tiles of 16 rows of a block with shared and with own keys; NS > 0: of a wave of a block with shared keys, whose waves share their steps.
-template <int E, int D, int NQS, int NQO, int NS, int OCC>
+// How a block takes its rows: KEYS, few of them, 16 * NQ rows whose keys the waves share out; ROWS, 64 * NQ rows, 16 * NQ for a wave.
+template <int E, int D, int NQ, int NS, bool NT>
+__device__ inline void prefix_block(const PrefixArgs& a, unsigned char* stages, const PartRows& w, int kvh) {
+  if constexpr (NS > 0) prefix_part_rows<E, D, NQ, NS>(a, stages, w, kvh);
+  else prefix_part<E, D, NQ, NT>(a, stages, w, kvh);
+}
+
+// NQS, NSS: of blocks with shared keys, the tiles of 16 rows (of a wave, if NSS > 0) and the steps of a ring that the waves share (0: each has its own);
+// NQO, NSO: of blocks with own keys.
+template <int E, int D, int NQS, int NSS, int NQO, int NSO, int OCC>
 __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(PrefixArgs a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char stages[(NS > PA_WAVES ? NS : PA_WAVES) * PrefixLane<E, D>::STAGE];
-  constexpr int ROWS = 16 * NQS * (NS > 0 ? PA_WAVES : 1);      // of a block with shared keys
+  constexpr int STEPS = (NSS > 0 && NSO > 0) ? (NSS > NSO ? NSS : NSO) : NSS > PA_WAVES ? NSS : PA_WAVES;
+  __shared__ __attribute__((aligned(1024))) unsigned char stages[STEPS * PrefixLane<E, D>::STAGE];
+  constexpr int ROWS = 16 * NQS * (NSS > 0 ? PA_WAVES : 1), OWN = 16 * NQO * (NSO > 0 ? PA_WAVES : 1);
   const int kvh = blockIdx.x % a.n_kv, group = a.n_heads / a.n_kv;
   int b = blockIdx.x / a.n_kv;
   PartRows w;
@@ -556,27 +568,32 @@ __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(Pr
     bool found = false;
     for (int g0 = 0; g0 < a.groups && !found; g0 += 64) {
       const int i = g0 + lane;
-      int keys = 0, tokens = 0, token0 = 0, r0 = 0;
+      int keys = 0, token0 = 0, end = 0, r0 = 0;
       if (i < a.groups) {
-        r0 = a.group_starts[i];
-        keys = min(a.group_keys[i], a.context_lens[r0]);     // (pages behind a request's context need not exist)
-        token0 = a.cu_seqlens[r0];
-        tokens = a.cu_seqlens[a.group_starts[i + 1]] - token0;
+        keys = a.group_keys[i];
+        r0 = token0 = a.group_starts[i];
+        end = a.group_starts[i + 1];
+        if (!a.single) {
+          token0 = a.cu_seqlens[r0];
+          end = a.cu_seqlens[end];
+        }
       }
-      const int blocks = keys > 0 ? (tokens * group + ROWS - 1) / ROWS : 0;
+      const int blocks = keys > 0 ? ((end - token0) * group + ROWS - 1) / ROWS : 0;
       int upto = blocks;
+      if (a.groups > 1) {
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(upto, d, 64);
-        if (lane >= d) upto += v;
+        for (int d = 1; d < 64; d <<= 1) {
+          const int v = __shfl_up(upto, d, 64);
+          if (lane >= d) upto += v;
+        }
       }
       const unsigned long long hit = __ballot(rb < upto);
       if (hit != 0) {
         const int src = (int)__builtin_ctzll(hit);
         w.row0 = (rb - __builtin_amdgcn_readlane(upto - blocks, src)) * ROWS;
-        w.end = __builtin_amdgcn_readlane(keys, src);
+        w.end = min(__builtin_amdgcn_readlane(keys, src), a.table_width << a.page_shift);
         w.token0 = __builtin_amdgcn_readlane(token0, src);
-        w.rows = min(ROWS, __builtin_amdgcn_readlane(tokens, src) * group - w.row0);
+        w.rows = min(ROWS, (__builtin_amdgcn_readlane(end, src) - w.token0) * group - w.row0);
         w.table = a.block_tables + (size_t)__builtin_amdgcn_readlane(r0, src) * a.table_width;
         found = true;
       }
@@ -587,68 +604,120 @@ __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(Pr
     if (w.first >= w.end) return;
     w.end = min(w.end, w.first + a.shared_steps * 32);
     w.limit0 = 0x7fffffff;
-    if constexpr (NS > 0) prefix_part_rows<E, D, NQS, NS>(a, stages, w, kvh);
-    else prefix_part<E, D, NQS, false>(a, stages, w, kvh);
+    prefix_block<E, D, NQS, NSS, false>(a, stages, w, kvh);
     return;
   }
   b -= a.shared_blocks;
   const int r = (b / a.own_rows) % a.requests, part = b / a.own_rows / a.requests;
-  const int t0 = a.cu_seqlens[r], tokens = a.cu_seqlens[r + 1] - t0;
-  const int ctx = a.context_lens[r], shared = a.shared_keys[r];
+  const int t0 = a.single ? r : a.cu_seqlens[r], tokens = a.single ? 1 : a.cu_seqlens[r + 1] - t0;
+  const int ctx = min(a.context_lens[r], a.table_width << a.page_shift), shared = a.shared_keys[r];
   w.token0 = t0;
-  w.row0 = (b % a.own_rows) * 16 * NQO;
-  w.rows = min(16 * NQO, tokens * group - w.row0);
+  w.row0 = (b % a.own_rows) * OWN;
+  w.rows = min(OWN, tokens * group - w.row0);
   w.first = part == 0 ? shared : (shared & ~15) + part * a.own_steps * 32;
   w.end = min(ctx, (shared & ~15) + (part + 1) * a.own_steps * 32);
   if (w.rows <= 0 || w.first >= w.end) return;
   w.limit0 = ctx - tokens;
   w.table = a.block_tables + (size_t)r * a.table_width;
   w.part = a.shared_parts + part;
-  prefix_part<E, D, NQO, true>(a, stages, w, kvh);
+  prefix_block<E, D, NQO, NSO, true>(a, stages, w, kvh);
 }
 
-// out[token, head, :] from a row's parts, in ascending order: those of its request's shared keys, then those of its own.  A wave a row; its lane
-// s holds part s's statistics.  Bound by one trip to memory: statistics and the first parts' sums are requested together.
-template <int E, int D>
+// out[token, head, :] from a row's parts, in a fixed order: those of its request's shared keys, then those of its own.  W waves a row, D / 4 lanes a
+// part, 16 bytes a lane; every wave works the weights out for itself (its lane s holds the statistics of parts s and 64 + s).  Bound by trips to
+// memory: which parts exist is asked beside all places' statistics (what stands in a place without a part is not used).
+template <int E, int D, int W>
 __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restrict__ sums, const float* __restrict__ stats,
                                                           const int* __restrict__ token_req, const int* __restrict__ context_lens,
                                                           const int* __restrict__ shared_keys, void* __restrict__ out, const float* __restrict__ sink,
-                                                          int rows, int heads, int shared_parts, int parts, int shared_steps, int own_steps) {
-  const int row = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+                                                          int rows, int heads, int shared_parts, int parts, int shared_steps, int own_steps, int single) {
+  constexpr int LANES = D / 4, GROUPS = W * 64 / LANES, AHEAD = 4;      // parts at a time, and how many times that is asked for at once
+  __shared__ __attribute__((aligned(16))) float red[W > 1 ? W * D : 4];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int row = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
   if (row >= rows) return;
-  const int token = row / heads, r = token_req[token];
+  const float* s = stats + (size_t)row * parts * 2;
+  float2 st[2] = {make_float2(-INFINITY, 0.f), make_float2(-INFINITY, 0.f)};
+  if (lane < parts) st[0] = *(const float2*)(s + lane * 2);
+  if (64 + lane < parts) st[1] = *(const float2*)(s + (64 + lane) * 2);
+  const float sunk = sink != nullptr ? sink[row % heads] : 0.f;
+  const int r = single ? row / heads : token_req[row / heads];
   const int shared = shared_keys[r], ctx = context_lens[r];
   const int n_shared = min(((shared + 31) / 32 + shared_steps - 1) / shared_steps, shared_parts);
-  const int n_own = min(((ctx - (shared & ~15) + 31) / 32 + own_steps - 1) / own_steps, parts - shared_parts);
-  const int n = n_shared + n_own;     // (lane i < n_shared: part i, else part shared_parts + i - n_shared)
-  const int part = lane < n_shared ? lane : shared_parts + lane - n_shared;
-  float2 st = make_float2(-INFINITY, 0.f);
-  if (lane < n) st = *(const float2*)(stats + ((size_t)row * parts + part) * 2);
-  const float top = wave_max(st.x), use = top == -INFINITY ? 0.f : top;
-  const float f = __builtin_amdgcn_exp2f(st.x - use);
-  float total = wave_sum(f * st.y);
-  if (sink != nullptr) total += __builtin_amdgcn_exp2f(fmaf(sink[row % heads], 1.4426950408889634f, -use));
-  constexpr int P = D >= 128 ? 2 : 1;     // elements a lane
-  float acc[P] = {};
-  const bool there = lane * P < D;
-  if (!there) return;
-  for (int i = 0; i < n; ++i) {
-    const float fi = lane_value(f, i);
-    const float* o = sums + ((size_t)row * parts + (i < n_shared ? i : shared_parts + i - n_shared)) * D + lane * P;
+  const int n = n_shared + min(((ctx - (shared & ~15) + 31) / 32 + own_steps - 1) / own_steps, parts - shared_parts);
+  // (part i of the n stands in place i, from n_shared on in place shared_parts + i - n_shared)
+  const int gap = shared_parts - n_shared;
+  const int mine = (W == 1 ? 0 : wave * (64 / LANES)) + lane / LANES;
+  const float* o = sums + (size_t)row * parts * D + (lane % LANES) * 4;
+  float4 val[AHEAD];
 #pragma unroll
-    for (int e = 0; e < P; ++e) acc[e] = fmaf(fi, o[e], acc[e]);
+  for (int k = 0; k < AHEAD; ++k) {
+    const int i = mine + k * GROUPS;
+    val[k] = i < n ? *(const float4*)(o + (size_t)(i < n_shared ? i : i + gap) * D) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
+  float top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int place = k * 64 + lane;
+    if (place >= n + gap || (place >= n_shared && place < shared_parts)) st[k] = make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, st[k].x);
+  }
+  top = wave_max(top);
+  const float use = top == -INFINITY ? 0.f : top;
+  const float f[2] = {__builtin_amdgcn_exp2f(st[0].x - use), __builtin_amdgcn_exp2f(st[1].x - use)};
+  float total = wave_sum(fmaf(f[0], st[0].y, f[1] * st[1].y));
+  if (sink != nullptr) total += __builtin_amdgcn_exp2f(fmaf(sunk, 1.4426950408889634f, -use));
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += AHEAD * GROUPS) {
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = i0 + mine + k * GROUPS, place = i < n_shared ? i : i + gap;
+      const float lo = __shfl(f[0], place & 63, 64), hi = __shfl(f[1], place & 63, 64);
+      const float w = i < n ? (place < 64 ? lo : hi) : 0.f;
+      acc.x = fmaf(w, val[k].x, acc.x);
+      acc.y = fmaf(w, val[k].y, acc.y);
+      acc.z = fmaf(w, val[k].z, acc.z);
+      acc.w = fmaf(w, val[k].w, acc.w);
+    }
+    if (i0 + AHEAD * GROUPS < n) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int i = i0 + AHEAD * GROUPS + mine + k * GROUPS;
+        val[k] = i < n ? *(const float4*)(o + (size_t)(i < n_shared ? i : i + gap) * D) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  }
+#pragma unroll
+  for (int d = LANES; d < 64; d <<= 1) {
+    acc.x += __shfl_xor(acc.x, d, 64);
+    acc.y += __shfl_xor(acc.y, d, 64);
+    acc.z += __shfl_xor(acc.z, d, 64);
+    acc.w += __shfl_xor(acc.w, d, 64);
+  }
+  if constexpr (W > 1) {
+    if (lane < LANES) *(float4*)(red + wave * D + lane * 4) = acc;
+    __syncthreads();
+    if (wave != 0) return;
+    acc = *(const float4*)(red + (lane % LANES) * 4);
+#pragma unroll
+    for (int v = 1; v < W; ++v) {
+      const float4 more = *(const float4*)(red + v * D + (lane % LANES) * 4);
+      acc.x += more.x;
+      acc.y += more.y;
+      acc.z += more.z;
+      acc.w += more.w;
+    }
+  }
+  if (lane >= LANES) return;
   const float inv = 1.0f / total;
-#pragma unroll
-  for (int e = 0; e < P; ++e) {
-    if constexpr (E == 2) ((bf16_t*)out)[(size_t)row * D + lane * P + e] = float_to_bf16(acc[e] * inv);
-    else ((float*)out)[(size_t)row * D + lane * P + e] = acc[e] * inv;
-  }
+  const size_t to = (size_t)row * D + lane * 4;
+  if constexpr (E == 2) from_float4((bf16_t*)out + to, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+  else from_float4((float*)out + to, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
-template <int E, int D, int NQS, int NQO, int NS>
+template <int E, int D, int NQS, int NSS, int NQO, int NSO>
 static int prefix_launch(const PrefixArgs& a, int blocks, hipStream_t s) {
-  prefix_attention_kernel<E, D, NQS, NQO, NS, E == 2 ? 2 : 1><<<blocks, PA_WAVES * 64, 0, s>>>(a);
+  prefix_attention_kernel<E, D, NQS, NSS, NQO, NSO, E == 2 ? 2 : 1><<<blocks, PA_WAVES * 64, 0, s>>>(a);
   return 0;
 }
 
@@ -656,14 +725,15 @@ template <int E, int D>
 static int prefix_sizes(const PrefixArgs& a, int blocks, int rows_shared, int rows_own, hipStream_t s) {
   constexpr int NS = E == 2 ? 4 : 2;
   if (rows_own == 16) {
-    if (rows_shared == 16) return prefix_launch<E, D, 1, 1, 0>(a, blocks, s);
-    if (rows_shared == 32) return prefix_launch<E, D, 2, 1, 0>(a, blocks, s);
-    if (rows_shared == 64) return prefix_launch<E, D, 1, 1, NS>(a, blocks, s);
-    if (rows_shared == 128) return prefix_launch<E, D, 2, 1, NS>(a, blocks, s);
-  } else if (rows_own == 32) {
-    if (rows_shared == 32) return prefix_launch<E, D, 2, 2, 0>(a, blocks, s);
-    if (rows_shared == 64) return prefix_launch<E, D, 1, 2, NS>(a, blocks, s);
-    if (rows_shared == 128) return prefix_launch<E, D, 2, 2, NS>(a, blocks, s);
+    if (rows_shared == 16) return prefix_launch<E, D, 1, 0, 1, 0>(a, blocks, s);
+    if (rows_shared == 32) return prefix_launch<E, D, 2, 0, 1, 0>(a, blocks, s);
+    if (rows_shared == 64) return prefix_launch<E, D, 1, NS, 1, 0>(a, blocks, s);
+    if (rows_shared == 128) return prefix_launch<E, D, 2, NS, 1, 0>(a, blocks, s);
+  } else if (rows_own == 64) {
+    if (rows_shared == 64) return prefix_launch<E, D, 1, NS, 1, NS>(a, blocks, s);
+    if (rows_shared == 128) return prefix_launch<E, D, 2, NS, 1, NS>(a, blocks, s);
+  } else if (rows_own == 128) {
+    if (rows_shared == 128) return prefix_launch<E, D, 2, NS, 2, NS>(a, blocks, s);
   }
   tp_set_error("prefix_attention: no kernel for blocks of %d and %d rows", rows_shared, rows_own);
   return 1;
@@ -671,8 +741,8 @@ static int prefix_sizes(const PrefixArgs& a, int blocks, int rows_shared, int ro
 
 // q [n, heads, dim] over pages of keys and transposed values (elements of dt), each request's context by its block table; out [n, heads * dim].
 // groups of requests share their first keys (group_starts [groups + 1], group_keys [groups], shared_keys [requests]: see PrefixArgs); every query
-// lies behind its request's shared keys.  shared_blocks: at least as many blocks of rows_shared rows (16, 32, 64 or 128) as all groups have; rows_own 16 or 32.  Parts of
-// shared_steps / own_steps steps of 32 keys, as many as there are at most.  scratch: n * heads * (shared_parts + own_parts) * (dim + 2) floats.
+// lies behind its request's shared keys.  shared_blocks: at least as many blocks of rows_shared rows (16, 32, 64 or 128) as all groups have; rows_own 16, 64 or 128.  Parts of
+// shared_steps / own_steps steps of 32 keys, as many as there are at most.  scratch: n * heads * (shared_parts + own_parts) * (dim + 2) + 2 floats, aligned to 16 bytes.
 extern "C" int tp_prefix_attention(const void* q, int dt, const void* k_cache, const void* v_cache, const int* block_tables, int table_width,
                                    const int* cu_seqlens, const int* context_lens, const int* token_req, const int* group_starts,
                                    const int* group_keys, const int* shared_keys, void* out, float* scratch, int n, int requests, int groups,
@@ -698,13 +768,14 @@ extern "C" int tp_prefix_attention(const void* q, int dt, const void* k_cache, c
   a.shared_keys = shared_keys;
   a.parts = shared_parts + own_parts;
   a.stats = scratch;
-  a.sums = scratch + (size_t)n * heads * a.parts * 2;
+  a.sums = scratch + ((size_t)n * heads * a.parts * 2 + 3) / 4 * 4;
   a.table_width = table_width;
   a.page_shift = __builtin_ctz(page_size);
   a.n_heads = heads;
   a.n_kv = kv_heads;
   a.groups = groups;
   a.requests = requests;
+  a.single = n == requests && max_q_len == 1;
   a.shared_rows = shared_blocks;
   a.shared_parts = shared_parts;
   a.own_rows = (int)(((long)max_q_len * (heads / kv_heads) + rows_own - 1) / rows_own);
@@ -725,9 +796,12 @@ extern "C" int tp_prefix_attention(const void* q, int dt, const void* k_cache, c
                                                                                             : prefix_sizes<4, 128>(a, (int)blocks, rows_shared, rows_own, s);
   if (rc != 0) return rc;
   TP_CHECK_LAUNCH("prefix_attention");
-  const int rows = n * heads, grid = (rows + 3) / 4;
-#define PA_JOIN(E, D) prefix_join_kernel<E, D><<<grid, 256, 0, s>>>(a.sums, a.stats, token_req, context_lens, shared_keys, out, sink, rows, heads, \
-                                                                     shared_parts, a.parts, shared_steps, own_steps)
+  // (a row of more than eight parts has four waves while the rows are not many: 1,024 rows of 32 parts 13.1 -> see below with one)
+  const int rows = n * heads;
+  const bool wide = a.parts > 8 && rows <= 4096;
+#define PA_JOIN_W(E, D, W) prefix_join_kernel<E, D, W><<<W == 1 ? (rows + 3) / 4 : rows, 256, 0, s>>>(a.sums, a.stats, token_req, context_lens, shared_keys, out, sink, \
+                                                                     rows, heads, shared_parts, a.parts, shared_steps, own_steps, a.single)
+#define PA_JOIN(E, D) (wide ? PA_JOIN_W(E, D, 4) : PA_JOIN_W(E, D, 1))
   if (dt == TP_BF16) {
     if (dim == 32) PA_JOIN(2, 32);
     else if (dim == 64) PA_JOIN(2, 64);
@@ -737,6 +811,7 @@ extern "C" int tp_prefix_attention(const void* q, int dt, const void* k_cache, c
     else if (dim == 64) PA_JOIN(4, 64);
     else PA_JOIN(4, 128);
   }
+#undef PA_JOIN_W
 #undef PA_JOIN
   TP_CHECK_LAUNCH("prefix_attention (join)");
   return 0;

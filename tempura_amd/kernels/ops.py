@@ -1540,7 +1540,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         return out
     group = heads // kvh
     rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts = _prefix_plan(n, r, group, kvh, max_q_len, shared, own, q.dtype)
-    scratch = torch.empty((n * heads * (shared_parts + own_parts) * (d + 2),), dtype=torch.float32, device=q.device)
+    scratch = torch.empty((n * heads * (shared_parts + own_parts) * (d + 2) + 2,), dtype=torch.float32, device=q.device)
     _call("tp_prefix_attention", _ptr(q), _dt(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), width, _ptr(cu_seqlens), _ptr(context_lens),
           _ptr(token_req), _ptr(shared.starts), _ptr(shared.keys), _ptr(shared.each), _ptr(out), _ptr(scratch), n, r, shared.groups, heads, kvh, d,
           page_size, float(scale), float(softcap), _ptr(sink), int(max_q_len), rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts,
@@ -1551,9 +1551,10 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
 def _prefix_plan(n, r, group, kvh, max_q_len, shared, own, dtype):
     most = min(n, shared.max_requests * max_q_len) * group
     rows = 16 if most <= 16 else 32 if most <= 32 else 64 if most <= 64 else 128
-    own_rows = 16 if max_q_len * group <= 16 else 32
+    own_rows = 16 if max_q_len * group <= 16 else 64 if max_q_len * group <= 64 else 128
+    rows = max(rows, own_rows)
     blocks = n * group // rows + shared.sharing
-    shared_steps, shared_parts = _prefix_parts(-(-shared.max_keys // 32), blocks * kvh, 48)
+    shared_steps, shared_parts = _prefix_parts(-(-shared.max_keys // 32), blocks * kvh, 112)
     own_steps, own_parts = _prefix_parts((own + 15 + 31) // 32, r * -(-max_q_len * group // own_rows) * kvh, 16)
     return rows, own_rows, blocks, shared_steps, shared_parts, own_steps, own_parts
 
