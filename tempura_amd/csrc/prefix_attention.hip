@@ -563,8 +563,10 @@ __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(Pr
   if (b < a.shared_blocks) {
     // which group's rows: a lane counts the blocks of one group, 64 groups at a time
     const int lane = threadIdx.x & 63;
-    int rb = b % a.shared_rows;
-    w.part = b / a.shared_rows;
+    // (a group's blocks of rows one behind the other, so that those that are not there come last: between the others they would take places
+    // of the round in which the blocks are handed to the CUs)
+    int rb = b / a.shared_parts;
+    w.part = b % a.shared_parts;
     bool found = false;
     for (int g0 = 0; g0 < a.groups && !found; g0 += 64) {
       const int i = g0 + lane;
@@ -726,7 +728,6 @@ static int prefix_sizes(const PrefixArgs& a, int blocks, int rows_shared, int ro
   constexpr int NS = E == 2 ? 4 : 2;
   if (rows_own == 16) {
     if (rows_shared == 16) return prefix_launch<E, D, 1, 0, 1, 0>(a, blocks, s);
-    if (rows_shared == 32) return prefix_launch<E, D, 2, 0, 1, 0>(a, blocks, s);
     if (rows_shared == 64) return prefix_launch<E, D, 1, NS, 1, 0>(a, blocks, s);
     if (rows_shared == 128) return prefix_launch<E, D, 2, NS, 1, 0>(a, blocks, s);
   } else if (rows_own == 64) {
@@ -741,7 +742,7 @@ static int prefix_sizes(const PrefixArgs& a, int blocks, int rows_shared, int ro
 
 // q [n, heads, dim] over pages of keys and transposed values (elements of dt), each request's context by its block table; out [n, heads * dim].
 // groups of requests share their first keys (group_starts [groups + 1], group_keys [groups], shared_keys [requests]: see PrefixArgs); every query
-// lies behind its request's shared keys.  shared_blocks: at least as many blocks of rows_shared rows (16, 32, 64 or 128) as all groups have; rows_own 16, 64 or 128.  Parts of
+// lies behind its request's shared keys.  shared_blocks: at least as many blocks of rows_shared rows (16, 64 or 128) as all groups have; rows_own 16, 64 or 128.  Parts of
 // shared_steps / own_steps steps of 32 keys, as many as there are at most.  scratch: n * heads * (shared_parts + own_parts) * (dim + 2) + 2 floats, aligned to 16 bytes.
 extern "C" int tp_prefix_attention(const void* q, int dt, const void* k_cache, const void* v_cache, const int* block_tables, int table_width,
                                    const int* cu_seqlens, const int* context_lens, const int* token_req, const int* group_starts,

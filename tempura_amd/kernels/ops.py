@@ -1487,6 +1487,7 @@ class SharedKeys:
         self.max_keys = max((v for _, v in runs), default=0)
         self.max_requests = max((c for c, v in runs if v), default=0)
         self.sharing = sum(1 for _, v in runs if v)
+        self._runs, self._plans = [(c, v) for c, v in runs if v], {}
         data = torch.tensor(starts + [v for _, v in runs] + [v for c, v in runs for _ in range(c)], dtype=torch.int32).to(device)
         self.starts, self.keys, self.each = data[: self.groups + 1], data[self.groups + 1: 2 * self.groups + 1], data[2 * self.groups + 1:]
 
@@ -1539,7 +1540,14 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if n == 0:
         return out
     group = heads // kvh
-    rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts = _prefix_plan(n, r, group, kvh, max_q_len, shared, own, q.dtype)
+    # (the most own keys rounded up, so that a growing step finds its plan again)
+    key = (n, group, kvh, max_q_len, -(-own // 256) * 256, d, q.dtype)
+    plan = shared._plans.get(key)
+    if plan is None:
+        if len(shared._plans) >= 256:
+            shared._plans.clear()
+        plan = shared._plans[key] = _prefix_plan(shared, r, *key)
+    rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts = plan
     scratch = torch.empty((n * heads * (shared_parts + own_parts) * (d + 2) + 2,), dtype=torch.float32, device=q.device)
     _call("tp_prefix_attention", _ptr(q), _dt(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), width, _ptr(cu_seqlens), _ptr(context_lens),
           _ptr(token_req), _ptr(shared.starts), _ptr(shared.keys), _ptr(shared.each), _ptr(out), _ptr(scratch), n, r, shared.groups, heads, kvh, d,
@@ -1548,22 +1556,41 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
-def _prefix_plan(n, r, group, kvh, max_q_len, shared, own, dtype):
+def _prefix_plan(shared: SharedKeys, r: int, n: int, group: int, kvh: int, max_q_len: int, own: int, dim: int, dtype: torch.dtype) -> tuple:
+    """(rows of a block with shared keys, with own keys, blocks of the former a key head and part, steps of 32 keys a part, parts, both for own keys)."""
+    f32 = dtype == torch.float32
+    # Rows: 16, whose keys the waves of a block share out, or 64 and 128, 16 and 32 a wave, which load a step once for all.  (8 requests of 4 heads a
+    # key head behind 2,048 keys: blocks of 16 / 64 rows 12.0 / 11.8 us; 32 behind 65,536: 64 / 128 92 / 75.)
     most = min(n, shared.max_requests * max_q_len) * group
-    rows = 16 if most <= 16 else 32 if most <= 32 else 64 if most <= 64 else 128
     own_rows = 16 if max_q_len * group <= 16 else 64 if max_q_len * group <= 64 else 128
-    rows = max(rows, own_rows)
-    blocks = n * group // rows + shared.sharing
-    shared_steps, shared_parts = _prefix_parts(-(-shared.max_keys // 32), blocks * kvh, 112)
-    own_steps, own_parts = _prefix_parts((own + 15 + 31) // 32, r * -(-max_q_len * group // own_rows) * kvh, 16)
-    return rows, own_rows, blocks, shared_steps, shared_parts, own_steps, own_parts
-
-
-def _prefix_parts(steps: int, blocks: int, most: int) -> tuple:
-    """(steps of 32 keys a part, parts) of keys of ``steps`` steps that ``blocks`` blocks a part walk."""
-    want = min(most, -(-512 // blocks), max(1, steps // 8))
-    per = -(-steps // max(1, want))
-    return per, -(-steps // per)
+    rows = max(own_rows, 16 if most <= 16 else 64 if most <= 64 else 128)
+    single = max_q_len == 1 and n == r
+    blocks = sum(-(-c * group // rows) for c, _ in shared._runs) if single else n * group // rows + shared.sharing
+    own_blocks = r * -(-max_q_len * group // own_rows)
+    # Parts: as long as the launch would take if it were spread evenly, less what a block takes to begin and the join.  A step takes a
+    # block that is alone on its CU step_us, two blocks twice that each; 5.5 TB/s is what single tokens' attention gets from memory.
+    # (64 requests behind 8,192 keys, 600 of their own: parts of 16 / 32 / 43 steps 50.6 / 45.7 / 53.7 us; 32 behind 65,536: 22 / 43 / 64 steps 85 / 75 / 78.)
+    step_us = (0.8 if rows == 128 else 0.55) * dim / 128 * (3 if f32 else 1)
+    slots = 256 if f32 and dim == 128 else 512
+    size = 4 if f32 else 2
+    row_steps = sum(-(-c * n // max(1, r) * group // rows) * -(-v // 32) for c, v in shared._runs) * kvh
+    own_steps = (own + 15 + 31) // 32
+    work_us = (2 * step_us * row_steps + own_blocks * kvh * (4 + own_steps * step_us / 4)) / slots
+    bytes_us = 2 * kvh * dim * size * (sum(v for _, v in shared._runs) + r * own / 2) / 5.5e6
+    steps = -(-shared.max_keys // 32)
+    per = max(8 if rows == 16 else 4, int(0.7 * max(work_us, bytes_us) / step_us))
+    parts = -(-steps // per)
+    # (More than a block a CU and less than one and a half is the worst of both: the CUs with two blocks set the time, 312 blocks 82 us, 384 75.  What is
+    # bound by its arithmetic fills the chip, but never a little more than one round: 56 blocks a part, 10 / 9 / 8 parts 52.5 / 44.0 / 46.0 us.)
+    if blocks * kvh * parts > slots // 2:
+        parts = max(parts, 3 * slots // 4 // (blocks * kvh))
+    if work_us > bytes_us:
+        parts = max(parts, min(-(-steps // 8), slots // (blocks * kvh)))
+    parts = max(1, min(parts, 112, slots // (blocks * kvh)))
+    per = -(-steps // parts)
+    # (own keys: two steps a wave, four where there are many blocks)
+    own_per = max(8 if own_blocks * kvh < 256 else 16, -(-own_steps // 16))
+    return rows, own_rows, blocks, per, -(-steps // per), own_per, -(-own_steps // own_per)
 
 
 def swiglu(gu: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
