@@ -44,10 +44,13 @@ __device__ inline void load8(const T* p, int left, float (&v)[8]) {
 }
 
 // ---- a few rows ------------------------------------------------------------------------------
-// A block takes one row and `cols` columns and works the row's low-rank values out for itself, those of its columns' slices.
-// grid: (ceil(N / cols), rows); block: 256.  v: LDS.
+// A block takes one row and `cols` columns and works the row's low-rank values out for itself, those of its columns' slices: one launch
+// instead of two, which costs each block rank * K elements of A from the L2 (128 KB with rank 16 and K = 4,096, 2 us of a CU's path), asked for by
+// sixteen waves at once.
+// grid: (ceil(N / cols), rows).  v: LDS.
+#define AD_ROW_THREADS 1024
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void adapter_rows_kernel(AdapterArgs a, int cols) {
+__global__ __launch_bounds__(AD_ROW_THREADS) void adapter_rows_kernel(AdapterArgs a, int cols) {
   extern __shared__ float v[];          // [slices of these columns, rank]
   const int row = blockIdx.y, n0 = blockIdx.x * cols, n1 = min(n0 + cols, a.N);
   const int slot = a.ids[row];
@@ -57,36 +60,48 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(AdapterArgs a, int co
   const int ranks = (s1 - s0 + 1) * a.rank;
   const T* x = (const T*)a.x + (size_t)row * a.K;
   const T* A = (const T*)a.a + ((size_t)slot * a.slices + s0) * a.rank * a.K;
-  for (int j = wave * 4; j < ranks; j += 16) {
-    float sum[4] = {};
+  // (a thread's column: its sum so far and its weights travel beside A)
+  const int n = n0 + (int)threadIdx.x;
+  const T* B = (const T*)a.b + ((size_t)slot * a.N + min(n, n1 - 1)) * a.rank;
+  float first[8];
+  load8<T, true>(B, 8, first);
+  const float scale = a.scale[slot];
+  float* y = a.y + (size_t)row * a.N;
+  const float old = n < n1 ? y[n] : 0.f;
+  constexpr int R = 2;                  // ranks of a wave at a time
+  for (int j = wave * R; j < ranks; j += R * (AD_ROW_THREADS / 64)) {
+    float sum[R] = {};
+#pragma unroll 4
     for (int k = lane * 8; k < a.K; k += 512) {
       float xv[8];
       load8<T, VEC>(x + k, a.K - k, xv);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < R; ++i) {
         float av[8];
         load8<T, VEC>(A + (size_t)(j + i) * a.K + k, a.K - k, av);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[i] = fmaf(av[e], xv[e], sum[i]);
       }
     }
-    const float total = wave_sums<4>(sum);      // (lane 16 i: the i-th)
-    if ((lane & 15) == 0) v[j + (lane >> 4)] = total;
+    const float total = wave_sums<R>(sum);      // (lane 32 i: the i-th)
+    if ((lane & 31) == 0) v[j + (lane >> 5)] = total;
   }
   __syncthreads();
-  const float scale = a.scale[slot];
-  for (int n = n0 + threadIdx.x; n < n1; n += 256) {
-    const T* B = (const T*)a.b + ((size_t)slot * a.N + n) * a.rank;
-    const float* vs = v + (slice_of(a, n) - s0) * a.rank;
+  for (int c = n; c < n1; c += AD_ROW_THREADS) {
+    const float* vs = v + (slice_of(a, c) - s0) * a.rank;
     float sum = 0.f;
     for (int j = 0; j < a.rank; j += 8) {
       float bv[8];
-      load8<T, true>(B + j, 8, bv);
+      if (c == n && j == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bv[e] = first[e];
+      } else {
+        load8<T, true>((const T*)a.b + ((size_t)slot * a.N + c) * a.rank + j, 8, bv);
+      }
 #pragma unroll
       for (int e = 0; e < 8; ++e) sum = fmaf(bv[e], vs[j + e], sum);
     }
-    float* y = a.y + (size_t)row * a.N + n;
-    *y = fmaf(scale, sum, *y);
+    y[c] = fmaf(scale, sum, c == n ? old : y[c]);
   }
 }
 
@@ -95,6 +110,7 @@ __global__ __launch_bounds__(256) void adapter_rows_kernel(AdapterArgs a, int co
 //   plan: [0] units; [4 ..] units of four ints (slot, first place, rows, 0); then the rows by place
 // (The order of a unit's rows follows the atomics below and may change from run to run: a row's sums do not hang on its place.)
 #define AD_UNIT 64
+#define AD_PARTS 8     // of K, at most
 typedef __bf16 ad_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float ad_f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int ad_u32x4 __attribute__((ext_vector_type(4)));
@@ -109,9 +125,16 @@ __global__ __launch_bounds__(1024) void adapter_plan_kernel(const int* __restric
   for (int i = threadIdx.x; i < slots; i += 1024) count[i] = 0;
   if (threadIdx.x == 0) base_rows = base_units = 0;
   __syncthreads();
-  for (int i = threadIdx.x; i < rows; i += 1024) {
-    const int s = ids[i];
-    if (s >= 0 && s < slots) atomicAdd(&count[s], 1);
+  // (neighbouring rows mostly have the same adapter: a wave counts its lanes with the same one and adds once)
+  for (int i0 = wave * 64; i0 < rows; i0 += 1024) {
+    const int i = i0 + lane, s = i < rows ? ids[i] : -1;
+    unsigned long long left = __ballot(s >= 0 && s < slots);
+    while (left != 0) {
+      const int src = (int)__builtin_ctzll(left), one = __builtin_amdgcn_readlane(s, src);
+      const unsigned long long same = __ballot(s == one);
+      if (lane == src) atomicAdd(&count[one], (int)__popcll(same));
+      left &= ~same;
+    }
   }
   __syncthreads();
   for (int s0 = 0; s0 < slots; s0 += 1024) {        // running sums over the slots, 1,024 at a time
@@ -149,9 +172,18 @@ __global__ __launch_bounds__(1024) void adapter_plan_kernel(const int* __restric
     }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < rows; i += 1024) {
-    const int s = ids[i];
-    if (s >= 0 && s < slots) order[atomicAdd(&count[s], 1)] = i;
+  for (int i0 = wave * 64; i0 < rows; i0 += 1024) {
+    const int i = i0 + lane, s = i < rows ? ids[i] : -1;
+    unsigned long long left = __ballot(s >= 0 && s < slots);
+    while (left != 0) {
+      const int src = (int)__builtin_ctzll(left), one = __builtin_amdgcn_readlane(s, src);
+      const unsigned long long same = __ballot(s == one);
+      int at = 0;
+      if (lane == src) at = atomicAdd(&count[one], (int)__popcll(same));
+      at = __builtin_amdgcn_readlane(at, src) + __builtin_amdgcn_mbcnt_hi((unsigned)(same >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)same, 0));
+      if (s == one) order[at] = i;
+      left &= ~same;
+    }
   }
   if (threadIdx.x == 0) *n_units = base_units;
 }
@@ -269,24 +301,34 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a, const in
     const int from = a.interleaved ? n0 : max(n0, s > 0 ? a.ends[s - 1] : 0), to = a.interleaved ? n1 : min(n1, a.ends[s]);
     for (int j0 = 0; j0 < a.rank; j0 += CHUNK) {
       __syncthreads();
-      for (int e = threadIdx.x; e < AD_UNIT * CHUNK; e += 256) {
-        const int row = e / CHUNK, j = e % CHUNK;
-        float sum = 0.f;
+      const int quads = min(CHUNK, (a.rank - j0 + STEP - 1) / STEP * STEP) / 4;      // (four values at a time; zeros up to a whole step)
+      for (int e = threadIdx.x; e < tiles * 16 * quads; e += 256) {
+        const int row = e / quads, j = e % quads * 4;
+        ad_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
         if (row < u.z && j0 + j < a.rank) {
           const float* p = v + ((size_t)u.y + row) * ranks + s * a.rank + j0 + j;
-          for (int k = 0; k < parts; ++k) sum += p[(size_t)k * a.rows * ranks];
+          ad_f32x4 part[AD_PARTS];
+#pragma unroll
+          for (int k = 0; k < AD_PARTS; ++k)
+            if (k < parts) part[k] = *(const ad_f32x4*)(p + (size_t)k * a.rows * ranks);
+#pragma unroll
+          for (int k = 0; k < AD_PARTS; ++k)
+            if (k < parts) sum += part[k];
           sum *= scale;
         }
         if constexpr (PIECES == 1) {
-          *(float*)(low[0] + row * ROW + j * 4) = sum;
+          *(ad_f32x4*)(low[0] + row * ROW + j * 4) = sum;
         } else {
-          float left = sum;
+          float left[4] = {sum[0], sum[1], sum[2], sum[3]};
 #pragma unroll
           for (int p = 0; p < PIECES; ++p) {
-            const unsigned bits = __builtin_bit_cast(unsigned, left) & 0xffff0000u;
-            *(uint16_t*)(low[p] + row * ROW + j * 2) = (uint16_t)(bits >> 16);
-            left -= __builtin_bit_cast(float, bits);
-            if (!(fabsf(sum) <= 3.4028234e38f)) left = 0.f;      // (infinite or no number: the first piece says it)
+            unsigned bits[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              bits[i] = __builtin_bit_cast(unsigned, left[i]) & 0xffff0000u;
+              left[i] = fabsf(sum[i]) <= 3.4028234e38f ? left[i] - __builtin_bit_cast(float, bits[i]) : 0.f;   // (infinite or no number: the first piece says it)
+            }
+            *(uint2*)(low[p] + row * ROW + j * 2) = make_uint2((bits[0] >> 16) | bits[1], (bits[2] >> 16) | bits[3]);
           }
         }
       }
@@ -375,7 +417,7 @@ extern "C" int tp_adapter_add(const int* ids, const void* x, int dt, const void*
   AdapterArgs g = {ids, x, a, b, scale, y, rows, K, N, slots, rank, slices, interleaved, {}};
   for (int i = 0; i < slices; ++i) g.ends[i] = ends[i];
   if (parts > 0) {
-    TP_REQUIRE(scratch != nullptr && slots <= 4096, "adapter_add: no room for a plan");
+    TP_REQUIRE(scratch != nullptr && slots <= 4096 && parts <= AD_PARTS, "adapter_add: no room for a plan");
     const int units = rows / AD_UNIT + (slots < rows ? slots : rows), ranks = rank * slices;
     int* n_units = (int*)scratch;
     int4* list = (int4*)scratch + 1;
@@ -402,17 +444,19 @@ extern "C" int tp_adapter_add(const int* ids, const void* x, int dt, const void*
     TP_CHECK_LAUNCH("adapter_add");
     return 0;
   }
-  const int cols = 256;
   TP_REQUIRE(rows <= 65535, "adapter_add: too many rows");
+  // (as many columns a block as threads, unless that leaves CUs without a block)
+  int cols = AD_ROW_THREADS;
+  while (cols > 256 && (long)rows * ((N + cols - 1) / cols) < 128) cols /= 2;
   const dim3 grid((N + cols - 1) / cols, rows);
   const size_t lds = (size_t)slices * rank * sizeof(float);
   TP_REQUIRE(lds <= 65536, "adapter_add: ranks of all slices beyond 16,384");
   if (dt == TP_BF16) {
-    if (vec) adapter_rows_kernel<bf16_t, true><<<grid, 256, lds, s>>>(g, cols);
-    else adapter_rows_kernel<bf16_t, false><<<grid, 256, lds, s>>>(g, cols);
+    if (vec) adapter_rows_kernel<bf16_t, true><<<grid, AD_ROW_THREADS, lds, s>>>(g, cols);
+    else adapter_rows_kernel<bf16_t, false><<<grid, AD_ROW_THREADS, lds, s>>>(g, cols);
   } else {
-    if (vec) adapter_rows_kernel<float, true><<<grid, 256, lds, s>>>(g, cols);
-    else adapter_rows_kernel<float, false><<<grid, 256, lds, s>>>(g, cols);
+    if (vec) adapter_rows_kernel<float, true><<<grid, AD_ROW_THREADS, lds, s>>>(g, cols);
+    else adapter_rows_kernel<float, false><<<grid, AD_ROW_THREADS, lds, s>>>(g, cols);
   }
   TP_CHECK_LAUNCH("adapter_add");
   return 0;
