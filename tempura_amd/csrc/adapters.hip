@@ -315,21 +315,26 @@ __global__ __launch_bounds__(256) void adapter_down_lds_kernel(AdapterArgs a, fl
   }
 }
 
-// y[row, n] = scale * B[n, :] . v[row, :] (zero without an adapter), or added to it: y^T[n, row], 16 columns and 16 rows a tile, so that a lane has four
-// neighbouring columns of its row.  The low-rank values, the sum of their parts times the scale, go through LDS once a block: float32 as they are; for bfloat16
-// weights as three bfloat16 pieces, the leading, middle and last eight bits, whose sum is the value, so nothing is rounded (2 rank columns
-// products more on matrix cores that wait for y anyway).  Bound by
-// writing y (and reading it, where it is added to).  A lane's weights of another slice than the one at hand are zero.
-// grid: (windows, blocks of cols columns, each)
-template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a, const float* __restrict__ v, int each, int parts, int cols, int write) {
+// y[row, n] = scale * B[n, :] . v[row, :] (zero without an adapter), or added to it: y^T[n, row], 16 columns and 16 rows a tile.  A wave has 16 * CT
+// columns, whose weights it keeps in registers for all of the window's rows; its tiles of 16 rows leave through LDS, so that rows are written in pieces of
+// 64 * CT bytes (straight from the tiles they would be 64 bytes of each of sixteen rows, one after the other in the same memory channel).
+// The low-rank values, the sum of their parts times the scale, go through LDS once a block: float32 as they are; for bfloat16 weights as three bfloat16
+// pieces, the leading, middle and last eight bits, whose sum is the value, so nothing is rounded (products more on matrix cores that wait for
+// memory anyway).  A lane's weights of another slice than the one at hand are zero.  Bound by writing y (and reading it, where it is added to).
+// grid: (windows, blocks of 64 * CT columns, each)
+template <typename T, int CT, bool VEC>
+__global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a, const float* __restrict__ v, int each, int parts, int write) {
   constexpr int P = 16 / sizeof(T), STEP = 4 * P;        // ranks a piece and a step
   constexpr int PIECES = sizeof(T) == 2 ? 3 : 1, CHUNK = 64, STEPS = CHUNK / STEP;      // ranks at a time
-  constexpr int ROW = CHUNK * sizeof(T) + 16;            // bytes of a row in LDS, a bank group more than the values
+  constexpr int ROW = CHUNK * sizeof(T) + 16;            // bytes of a row of low-rank values in LDS, a bank group more than the values
+  constexpr int WIDE = 16 * CT, OUT = WIDE + 4;          // columns of a wave, and floats of a row on its way out
+  constexpr int MOST = AD_WINDOW * CHUNK / 4 / 256;
   __shared__ __attribute__((aligned(16))) unsigned char low[PIECES][AD_WINDOW * ROW];
+  __shared__ __attribute__((aligned(16))) float tile[4][16 * OUT];
   __shared__ int order[AD_WINDOW];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-  const int n0 = blockIdx.y * cols, n1 = min(n0 + cols, a.N), ranks = a.rank * a.slices;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
+  const int n0 = blockIdx.y * 4 * WIDE, n1 = min(n0 + 4 * WIDE, a.N), ranks = a.rank * a.slices;
+  const int w0 = n0 + wave * WIDE, w1 = min(w0 + WIDE, a.N);
   const int s0 = a.interleaved ? 0 : slice_of(a, n0), s1 = a.interleaved ? 1 : slice_of(a, n1 - 1);
   for (int which = blockIdx.z;; which += each) {
     int slot;
@@ -347,105 +352,103 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a, const fl
     }
     const int tiles = (count + 15) >> 4;
     const float scale = a.scale[slot];
-    size_t yrow[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) yrow[t] = (size_t)order[min(t * 16 + c, count - 1)] * a.N;
     for (int s = s0; s <= s1; ++s) {
-      const int from = a.interleaved ? n0 : max(n0, s > 0 ? a.ends[s - 1] : 0), to = a.interleaved ? n1 : min(n1, a.ends[s]);
+      const int from = a.interleaved ? w0 : max(w0, s > 0 ? a.ends[s - 1] : 0), to = a.interleaved ? w1 : min(w1, a.ends[s]);     // this wave's columns
       for (int j0 = 0; j0 < a.rank; j0 += CHUNK) {
         const bool add = !write || j0 > 0 || (a.interleaved && s > 0);
-        __syncthreads();
-        const int quads = min(CHUNK, (a.rank - j0 + STEP - 1) / STEP * STEP) / 4;      // (four values at a time; zeros up to a whole step)
-        for (int e = threadIdx.x; e < tiles * 16 * quads; e += 256) {
-          const int row = e / quads, j = e % quads * 4;
-          ad_f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-          if (row < count && j0 + j < a.rank) {
-            const float* p = v + (size_t)order[min(row, count - 1)] * ranks + s * a.rank + j0 + j;
-            ad_f32x4 part[AD_PARTS];
+        ad_u32x4 bf[CT][STEPS];
 #pragma unroll
-            for (int k = 0; k < AD_PARTS; ++k)
-              if (k < parts) part[k] = *(const ad_f32x4*)(p + (size_t)k * a.rows * ranks);
+        for (int i = 0; i < CT; ++i) {
+          const int col = w0 + 16 * i + c;
+          const bool mine = col >= from && col < to && (!a.interleaved || ((col >> 3) & 1) == s);
+          const T* B = (const T*)a.b + ((size_t)slot * a.N + min(col, a.N - 1)) * a.rank;
 #pragma unroll
-            for (int k = 0; k < AD_PARTS; ++k)
-              if (k < parts) sum += part[k];
-            sum *= scale;
+          for (int k = 0; k < STEPS; ++k) {
+            const int j = j0 + k * STEP + g * P;
+            bf[i][k] = (ad_u32x4){0, 0, 0, 0};
+            if (mine && j < a.rank) bf[i][k] = *(const ad_u32x4*)(B + j);
           }
+        }
+        __syncthreads();
+        // (four values at a time, zeros up to a whole step of ranks; two parts of all of a thread's values are asked for together)
+        const int quads = min(CHUNK, (a.rank - j0 + STEP - 1) / STEP * STEP) / 4, items = tiles * 16 * quads;
+        ad_f32x4 sum[MOST];
+#pragma unroll
+        for (int it = 0; it < MOST; ++it) sum[it] = (ad_f32x4){0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < parts; k += 2) {
+          ad_f32x4 part[2][MOST];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int it = 0; it < MOST; ++it) {
+              const int e = threadIdx.x + it * 256, row = e / quads, j = j0 + e % quads * 4;
+              part[h][it] = (ad_f32x4){0.f, 0.f, 0.f, 0.f};
+              if (e < items && row < count && j < a.rank && k + h < parts)
+                part[h][it] = *(const ad_f32x4*)(v + ((size_t)(k + h) * a.rows + order[row]) * ranks + s * a.rank + j);
+            }
+#pragma unroll
+          for (int it = 0; it < MOST; ++it) sum[it] = (sum[it] + part[0][it]) + part[1][it];
+        }
+#pragma unroll
+        for (int it = 0; it < MOST; ++it) {
+          const int e = threadIdx.x + it * 256, row = e / quads, j = e % quads * 4;
+          if (e >= items) break;
+          float left[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) left[i] = sum[it][i] * scale;
           if constexpr (PIECES == 1) {
-            *(ad_f32x4*)(low[0] + row * ROW + j * 4) = sum;
+            *(float4*)(low[0] + row * ROW + j * 4) = make_float4(left[0], left[1], left[2], left[3]);
           } else {
-            float left[4] = {sum[0], sum[1], sum[2], sum[3]};
 #pragma unroll
             for (int p = 0; p < PIECES; ++p) {
               unsigned bits[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
+                const bool finite = fabsf(left[i]) <= 3.4028234e38f;      // (else the first piece says it)
                 bits[i] = __builtin_bit_cast(unsigned, left[i]) & 0xffff0000u;
-                left[i] = fabsf(sum[i]) <= 3.4028234e38f ? left[i] - __builtin_bit_cast(float, bits[i]) : 0.f;   // (infinite or no number: the first piece says it)
+                left[i] = finite ? left[i] - __builtin_bit_cast(float, bits[i]) : 0.f;
               }
               *(uint2*)(low[p] + row * ROW + j * 2) = make_uint2((bits[0] >> 16) | bits[1], (bits[2] >> 16) | bits[3]);
             }
           }
         }
         __syncthreads();
-        for (int n = (from & ~15) + wave * 32; n < to; n += 128) {
-          // 32 columns: two tiles
-          ad_f32x4 acc[2][4], old[2][4];
-          ad_u32x4 bf[2][STEPS];
+        if (from >= to) continue;
+        for (int t = 0; t < tiles; ++t) {
+          ad_f32x4 acc[CT];
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int col = n + 16 * i + c;
-            const bool mine = col >= from && col < to && (!a.interleaved || ((col >> 3) & 1) == s);
-            const T* B = (const T*)a.b + ((size_t)slot * a.N + min(col, a.N - 1)) * a.rank;
-#pragma unroll
-            for (int k = 0; k < STEPS; ++k) {
-              const int j = j0 + k * STEP + g * P;
-              bf[i][k] = mine && j < a.rank ? *(const ad_u32x4*)(B + j) : (ad_u32x4){0, 0, 0, 0};
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              acc[i][t] = old[i][t] = (ad_f32x4){0.f, 0.f, 0.f, 0.f};
-              const int col = n + 16 * i + 4 * g;
-              if (VEC) {
-                if (add && t < tiles && col < a.N) old[i][t] = *(const ad_f32x4*)(a.y + yrow[t] + col);
-              } else if (add && t < tiles) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) old[i][t][r] = col + r < a.N ? a.y[yrow[t] + col + r] : 0.f;
-              }
-            }
+          for (int i = 0; i < CT; ++i) acc[i] = (ad_f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < STEPS; ++k) {
             if (j0 + k * STEP >= a.rank) break;
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
-              if (t < tiles) {
+            for (int p = 0; p < PIECES; ++p) {
+              const ad_u32x4 lf = *(const ad_u32x4*)(low[p] + (t * 16 + c) * ROW + (k * 4 + g) * 16);
 #pragma unroll
-                for (int p = 0; p < PIECES; ++p) {
-                  const ad_u32x4 lf = *(const ad_u32x4*)(low[p] + (t * 16 + c) * ROW + (k * 4 + g) * 16);
-#pragma unroll
-                  for (int i = 0; i < 2; ++i) mfma_piece<T>(bf[i][k], lf, acc[i][t]);
-                }
-              }
-          }
-#pragma unroll
-          for (int t = 0; t < 4; ++t)
-            if (t * 16 + c < count) {
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int col = n + 16 * i + 4 * g;
-                // (a tile that reaches into the columns of another wave, slice or block leaves those alone)
-                const bool all = col >= from && col + 4 <= to;
-                if (VEC && all) {
-                  *(ad_f32x4*)(a.y + yrow[t] + col) = old[i][t] + acc[i][t];
-                } else {
-#pragma unroll
-                  for (int r = 0; r < 4; ++r)
-                    if (col + r >= from && col + r < to) a.y[yrow[t] + col + r] = old[i][t][r] + acc[i][t][r];
-                }
-              }
+              for (int i = 0; i < CT; ++i) mfma_piece<T>(bf[i][k], lf, acc[i]);
             }
+          }
+          // (the wave's own part of LDS: its writes and reads follow each other without a barrier)
+#pragma unroll
+          for (int i = 0; i < CT; ++i) *(ad_f32x4*)(tile[wave] + c * OUT + i * 16 + 4 * g) = acc[i];
+          __builtin_amdgcn_wave_barrier();
+          constexpr int LANES = WIDE / 4, ROWS = 64 / LANES;      // of a row; rows at a time
+#pragma unroll
+          for (int i = 0; i < 16 / ROWS; ++i) {
+            const int row = i * ROWS + lane / LANES, col = lane % LANES * 4;
+            if (t * 16 + row >= count) continue;
+            ad_f32x4 value = *(const ad_f32x4*)(tile[wave] + row * OUT + col);
+            float* y = a.y + (size_t)order[t * 16 + row] * a.N + w0 + col;
+            if (VEC && w0 + col >= from && w0 + col + 4 <= to) {
+              if (add) value += *(const ad_f32x4*)y;
+              *(ad_f32x4*)y = value;
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (w0 + col + r >= from && w0 + col + r < to) y[r] = add ? y[r] + value[r] : value[r];
+            }
+          }
+          __builtin_amdgcn_wave_barrier();
         }
       }
     }
@@ -471,16 +474,22 @@ static void adapter_many(const AdapterArgs& g, int parts, int vec, int write, fl
   if (vec && g.K % SK == 0) {
     if (rt == 1) adapter_down_lds_kernel<T, 1, 6><<<down, 256, 0, s>>>(g, v, each, part_k);
     else if (rt == 2) adapter_down_lds_kernel<T, 2, 6><<<down, 256, 0, s>>>(g, v, each, part_k);
-    else adapter_down_lds_kernel<T, 4, 5><<<down, 256, 0, s>>>(g, v, each, part_k);
+    else adapter_down_lds_kernel<T, 4, 4><<<down, 256, 0, s>>>(g, v, each, part_k);
   } else if (vec) {
     adapter_down<T, true>(g, down, rt, v, each, part_k, s);
   } else {
     adapter_down<T, false>(g, down, rt, v, each, part_k, s);
   }
-  const int cols = 512;
-  const dim3 up(windows, (g.N + cols - 1) / cols, each);
-  if (g.N % 4 == 0 && ((uintptr_t)g.y & 15) == 0) adapter_up_kernel<T, true><<<up, 256, 0, s>>>(g, v, each, down.y, cols, write);
-  else adapter_up_kernel<T, false><<<up, 256, 0, s>>>(g, v, each, down.y, cols, write);
+  // (128 columns a wave, unless that leaves CUs without a block: then 32)
+  const bool y16 = g.N % 4 == 0 && ((uintptr_t)g.y & 15) == 0, wide = (long)windows * ((g.N + 511) / 512) >= 192;
+  const dim3 up(windows, wide ? (g.N + 511) / 512 : (g.N + 127) / 128, each);
+  if (wide) {
+    if (y16) adapter_up_kernel<T, 8, true><<<up, 256, 0, s>>>(g, v, each, down.y, write);
+    else adapter_up_kernel<T, 8, false><<<up, 256, 0, s>>>(g, v, each, down.y, write);
+  } else {
+    if (y16) adapter_up_kernel<T, 2, true><<<up, 256, 0, s>>>(g, v, each, down.y, write);
+    else adapter_up_kernel<T, 2, false><<<up, 256, 0, s>>>(g, v, each, down.y, write);
+  }
 }
 
 // y [rows, N] float32 += the adapters' share.  a [slots, slices * rank, K], b [slots, N, rank] of dt, rank a multiple of 8; vec: K is a multiple of
