@@ -744,12 +744,15 @@ static int prefix_sizes(const PrefixArgs& a, int blocks, int rows_shared, int ro
 // groups of requests share their first keys (group_starts [groups + 1], group_keys [groups], shared_keys [requests]: see PrefixArgs); every query
 // lies behind its request's shared keys.  shared_blocks: at least as many blocks of rows_shared rows (16, 64 or 128) as all groups have; rows_own 16, 64 or 128.  Parts of
 // shared_steps / own_steps steps of 32 keys, as many as there are at most.  scratch: n * heads * (shared_parts + own_parts) * (dim + 2) + 2 floats, aligned to 16 bytes.
-extern "C" int tp_prefix_attention(const void* q, int dt, const void* k_cache, const void* v_cache, const int* block_tables, int table_width,
-                                   const int* cu_seqlens, const int* context_lens, const int* token_req, const int* group_starts,
-                                   const int* group_keys, const int* shared_keys, void* out, float* scratch, int n, int requests, int groups,
-                                   int heads, int kv_heads, int dim, int page_size, float scale, float softcap, const float* sink, int max_q_len,
-                                   int rows_shared, int rows_own, int shared_blocks, int shared_steps, int shared_parts, int own_steps, int own_parts,
+// sizes: element type, table width, n, requests, groups, heads, key heads, dim, page size, the most tokens of a request, rows_shared, rows_own,
+// shared_blocks, shared_steps, shared_parts, own_steps, own_parts.
+extern "C" int tp_prefix_attention(const void* q, const void* k_cache, const void* v_cache, const int* block_tables, const int* cu_seqlens,
+                                   const int* context_lens, const int* token_req, const int* group_starts, const int* group_keys,
+                                   const int* shared_keys, void* out, float* scratch, const float* sink, const int* sizes, float scale, float softcap,
                                    hipStream_t s) {
+  const int dt = sizes[0], table_width = sizes[1], n = sizes[2], requests = sizes[3], groups = sizes[4], heads = sizes[5], kv_heads = sizes[6],
+            dim = sizes[7], page_size = sizes[8], max_q_len = sizes[9], rows_shared = sizes[10], rows_own = sizes[11], shared_blocks = sizes[12],
+            shared_steps = sizes[13], shared_parts = sizes[14], own_steps = sizes[15], own_parts = sizes[16];
   if (n <= 0 || requests <= 0) return 0;
   TP_REQUIRE(dt == TP_BF16 || dt == TP_F32, "prefix_attention: unsupported element type");
   TP_REQUIRE(dim == 32 || dim == 64 || dim == 128, "prefix_attention: heads of 32, 64 or 128 elements");

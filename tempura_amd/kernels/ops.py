@@ -1520,6 +1520,39 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         return _backend.prefix_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, shared, max_q_len,
                                          max_context_len, max_own_len, num_single, sink, softcap)
     _dev_ok(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, sink, shared.starts)
+    own = int(max_context_len if max_own_len is None else max_own_len)
+    _need(0 < own <= max(1, max_context_len), "prefix_attention: max_own_len must be between 1 and the longest context")
+    _need(softcap >= 0, "prefix_attention: softcap must not be negative")
+    # (what a call is refused for by its shapes, and how it is laid out, is found once for calls that are alike; the most own keys rounded up, so that
+    # a growing step finds its plan again)
+    key = (q.shape, k_cache.shape, v_cache.shape, block_tables.shape, q.dtype, k_cache.dtype, v_cache.dtype, max_q_len, max_context_len, (own + 255) // 256)
+    plan = shared._plans.get(key)
+    if plan is None:
+        plan = _prefix_checked(q, k_cache, v_cache, block_tables, shared, int(max_q_len), int(max_context_len), (own + 255) // 256 * 256)
+        if len(shared._plans) >= 256:
+            shared._plans.clear()
+        shared._plans[key] = plan
+    n, r, heads, sizes, room = plan
+    if not (cu_seqlens.dtype == context_lens.dtype == token_req.dtype == block_tables.dtype == torch.int32 and cu_seqlens.numel() > r
+            and context_lens.numel() >= r and token_req.numel() >= n):
+        raise KernelError("prefix_attention: block_tables, cu_seqlens [r + 1], context_lens [r] and token_req [n] must be int32")
+    if sink is not None:
+        _need(sink.dtype == torch.float32 and sink.numel() == heads, "prefix_attention: sink must be float32 [heads]")
+    if sizes is None:
+        return paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, 0, max_q_len, max_context_len,
+                               num_single, sink=sink, softcap=softcap)
+    out = torch.empty((n, heads * q.shape[2]), dtype=q.dtype, device=q.device)
+    if n == 0:
+        return out
+    scratch = torch.empty((room,), dtype=torch.float32, device=q.device)
+    _call("tp_prefix_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), cu_seqlens.data_ptr(), context_lens.data_ptr(),
+          token_req.data_ptr(), shared.starts.data_ptr(), shared.keys.data_ptr(), shared.each.data_ptr(), out.data_ptr(), scratch.data_ptr(), _ptr(sink),
+          sizes, scale, softcap, _stream())
+    return out
+
+
+def _prefix_checked(q, k_cache, v_cache, block_tables, shared: SharedKeys, max_q_len: int, max_context_len: int, own: int) -> tuple:
+    """(tokens, requests, heads, the kernel's sizes or None where ``paged_attention`` runs, floats of scratch) of calls with these shapes."""
     _need(q.dim() == 3 and k_cache.dim() == 4 and v_cache.dim() == 4, "prefix_attention: bad operand ranks")
     n, heads, d = q.shape
     pages, kvh, page_size, d2 = k_cache.shape
@@ -1527,42 +1560,19 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     _need(tuple(v_cache.shape) == (pages, kvh, vd, page_size), "prefix_attention: v cache must be [pages, kv_heads, value_dim, page_size]")
     _need(d == d2 and kvh > 0 and heads % kvh == 0, "prefix_attention: heads of q and cache differ")
     _need(q.dtype == k_cache.dtype == v_cache.dtype, "prefix_attention: q and cache dtypes differ")
-    _need(block_tables.dim() == 2 and block_tables.dtype == torch.int32, "prefix_attention: block_tables must be int32 [r, width]")
+    _need(block_tables.dim() == 2, "prefix_attention: block_tables must be int32 [r, width]")
     r, width = block_tables.shape
     if shared.requests != r:
         raise KernelError(f"prefix_attention: runs of {shared.requests} requests for a batch of {r}")
-    _i32(cu_seqlens, r + 1, "cu_seqlens")
-    _i32(context_lens, r, "context_lens") if r else None
-    _i32(token_req, n, "token_req") if n else None
     _need(n >= r and max_q_len >= 1, "prefix_attention: every request brings at least one token")
     _need(max_context_len <= width * page_size, "prefix_attention: block table narrower than the longest context")
     _need(shared.max_keys < max(1, max_context_len), "prefix_attention: a request's new tokens must lie behind its shared keys")
-    _need(softcap >= 0, "prefix_attention: softcap must not be negative")
-    own = int(max_context_len if max_own_len is None else max_own_len)
-    _need(0 < own <= max(1, max_context_len), "prefix_attention: max_own_len must be between 1 and the longest context")
-    if sink is not None:
-        _need(sink.dtype == torch.float32 and sink.numel() == heads, "prefix_attention: sink must be float32 [heads]")
     if shared.max_keys == 0 or not prefix_attention_ok(q.dtype, heads, kvh, d, vd, page_size, max_q_len):
-        return paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, 0, max_q_len, max_context_len,
-                               num_single, sink=sink, softcap=softcap)
-    out = torch.empty((n, heads * vd), dtype=q.dtype, device=q.device)
-    if n == 0:
-        return out
-    group = heads // kvh
-    # (the most own keys rounded up, so that a growing step finds its plan again)
-    key = (n, group, kvh, max_q_len, -(-own // 256) * 256, d, q.dtype)
-    plan = shared._plans.get(key)
-    if plan is None:
-        if len(shared._plans) >= 256:
-            shared._plans.clear()
-        plan = shared._plans[key] = _prefix_plan(shared, r, *key)
-    rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts = plan
-    scratch = torch.empty((n * heads * (shared_parts + own_parts) * (d + 2) + 2,), dtype=torch.float32, device=q.device)
-    _call("tp_prefix_attention", _ptr(q), _dt(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables), width, _ptr(cu_seqlens), _ptr(context_lens),
-          _ptr(token_req), _ptr(shared.starts), _ptr(shared.keys), _ptr(shared.each), _ptr(out), _ptr(scratch), n, r, shared.groups, heads, kvh, d,
-          page_size, float(scale), float(softcap), _ptr(sink), int(max_q_len), rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts,
-          _stream())
-    return out
+        return n, r, heads, None, 0
+    rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts = _prefix_plan(shared, r, n, heads // kvh, kvh, max_q_len, own, d, q.dtype)
+    sizes = (_dt(q), width, n, r, shared.groups, heads, kvh, d, page_size, max_q_len, rows_shared, rows_own, blocks, shared_steps, shared_parts,
+             own_steps, own_parts)
+    return n, r, heads, (ctypes.c_int * len(sizes))(*sizes), n * heads * (shared_parts + own_parts) * (d + 2) + 2
 
 
 def _prefix_plan(shared: SharedKeys, r: int, n: int, group: int, kvh: int, max_q_len: int, own: int, dim: int, dtype: torch.dtype) -> tuple:
