@@ -17,6 +17,7 @@ import torch
 from ..config import load_config
 from ..kernels import ops
 from ..sampling import Sampler, SamplingParams
+from ..weights.adapters import read_adapter
 from .loading import load_model, parse_dtype, random_model
 from .model import CausalLM
 from .runner import ModelRunner, StepEntry
@@ -30,7 +31,8 @@ class Engine:
                  gpu_memory_utilization: float = 0.9, max_batch_size: int = 64,
                  max_seq_len: Optional[int] = None, max_num_batched_tokens: int = 2048,
                  prefill_chunk_size: int = 512, device: str = "cuda:0", use_graph: bool = True,
-                 chain_steps: bool = True, fill_budget: bool = True, admit_headroom: Optional[float] = 0.02):
+                 chain_steps: bool = True, fill_budget: bool = True, admit_headroom: Optional[float] = 0.02,
+                 max_adapters: int = 0, max_adapter_rank: int = 16):
         """``model``: a folder with config.json and safetensors, or (with ``random_weights``) a typed
         configuration such as ``LlamaConfig``/``PRESETS[name]``.
         ``kv_pages``: cache pages per group; by default as many as ``gpu_memory_utilization`` of the
@@ -43,7 +45,9 @@ class Engine:
         tokens, so the GPU does not wait for the host between steps; a request that ends on the token just
         read has then one row computed for nothing.  What the caller sees does not change.
         ``admit_headroom``: share of the cache pages that an admission leaves free beside running requests (None:
-        a request comes in as soon as its first portion fits; see ``SchedulerConfig.admit_headroom``)."""
+        a request comes in as soon as its first portion fits; see ``SchedulerConfig.admit_headroom``).
+        ``max_adapters``: how many low-rank adapters of up to ``max_adapter_rank`` may be loaded at a time (``load_adapter``); the room for
+        them is taken at once, and the model's norms run as kernels of their own (0: neither)."""
         self.device = torch.device(device)
         if isinstance(model, str):
             if random_weights:
@@ -57,6 +61,13 @@ class Engine:
                 raise ValueError("a configuration without a folder needs random_weights=True")
             self.model = random_model(model, seed, dtype, device)
         spec = self.model.spec
+        if max_adapters < 0 or max_adapter_rank < 1:
+            raise ValueError("max_adapters must not be negative, max_adapter_rank must be positive")
+        self._adapter_targets = self.model.enable_adapters(int(max_adapters), int(max_adapter_rank)) if max_adapters else {}
+        if max_adapters and not self._adapter_targets:
+            raise ValueError("no projection of this model takes adapters")
+        self._adapters: Dict[str, int] = {}          # name -> slot
+        self._free_adapters = list(range(int(max_adapters)))[::-1]
         self.max_seq_len = min(int(max_seq_len or spec.max_positions), spec.max_positions)
         self.page_size = int(page_size)
         if kv_pages is None:
@@ -98,16 +109,57 @@ class Engine:
         budget = int(free * utilization) - workspace - state_bytes
         return max(1, min(pages_cap, budget // per_page))
 
+    # ---- adapters ------------------------------------------------------------
+    def load_adapter(self, name: str, source: Union[str, Dict[str, Tuple[torch.Tensor, torch.Tensor]]], scale: Optional[float] = None) -> None:
+        """Load a low-rank adapter that requests may then name (``add_request``): a folder (``adapter_config.json`` and
+        ``adapter_model.safetensors``, weights/adapters.py) or a dict of base tensor name -> (A [rank, inputs], B [outputs, rank]) with its
+        ``scale`` (for a folder None: the configuration's).  Every fault is reported in one error and nothing is loaded then."""
+        if name in self._adapters:
+            raise ValueError(f"adapter {name!r} is loaded already")
+        if not self._free_adapters:
+            raise ValueError(f"{len(self._adapters)} adapters are loaded, there is room for no more (max_adapters)")
+        if isinstance(source, str):
+            pairs, said = read_adapter(source)
+            scale = said if scale is None else scale
+        else:
+            pairs = dict(source)
+        if scale is None:
+            raise ValueError("an adapter from tensors needs its scale")
+        faults = []
+        for tensor, pair in pairs.items():
+            where = self._adapter_targets.get(tensor)
+            fault = "no projection that takes adapters" if where is None else where[0].adapters[where[1]].fault(where[2], pair)
+            if fault:
+                faults.append(f"{tensor}: {fault}")
+        if faults or not pairs:
+            raise ValueError(f"adapter {name!r}: " + ("; ".join(faults) or "no tensors"))
+        slot = self._free_adapters.pop()
+        for part in {id(w[0]): w[0] for w in self._adapter_targets.values()}.values():
+            part.set_adapter(slot, pairs, float(scale))
+        self._adapters[name] = slot
+
+    def unload_adapter(self, name: str) -> None:
+        """Give an adapter's place back; refused while a request that names it is unfinished."""
+        if name not in self._adapters:
+            raise KeyError(f"adapter {name!r} is not loaded (loaded: {sorted(self._adapters)})")
+        slot = self._adapters[name]
+        busy = [rid for rid, req in self._requests.items() if req.state != RequestState.FINISHED and self.runner.adapter_of.get(rid) == slot]
+        if busy:
+            raise ValueError(f"adapter {name!r} is in use by request {busy[0]!r}")
+        self._free_adapters.append(self._adapters.pop(name))
+
     # ---- requests ------------------------------------------------------------
     def add_request(self, prompt_ids: Sequence[int], params: Optional[SamplingParams] = None,
-                    rid: Optional[Hashable] = None, logprobs_top_n: Optional[int] = None) -> Hashable:
+                    rid: Optional[Hashable] = None, logprobs_top_n: Optional[int] = None, adapter: Optional[str] = None) -> Hashable:
         """Queue a request.  With ``logprobs_top_n`` (0..20) every generated token gets a ``TokenLogprob``
-        record in ``request(rid).logprobs``."""
+        record in ``request(rid).logprobs``.  ``adapter``: the name of a loaded adapter (``load_adapter``)."""
         params = params or SamplingParams()
         if rid is None:
             rid = next(self._ids)
         if rid in self._requests and self._requests[rid].state != RequestState.FINISHED:
             raise ValueError(f"request id {rid!r} is in use")
+        if adapter is not None and adapter not in self._adapters:
+            raise ValueError(f"adapter {adapter!r} is not loaded (loaded: {sorted(self._adapters)})")
         vocab = self.model.spec.vocab_size
         for t in prompt_ids:
             if t < 0 or t >= vocab:
@@ -117,6 +169,9 @@ class Engine:
                       logprobs_top_n=logprobs_top_n)
         self.scheduler.add_request(req)
         self._requests[rid] = req
+        self.runner.adapter_of.pop(rid, None)
+        if adapter is not None and req.state != RequestState.FINISHED:
+            self.runner.adapter_of[rid] = self._adapters[adapter]
         self.counters["prompt_tokens"] += len(req.prompt)
         return rid
 
@@ -184,6 +239,7 @@ class Engine:
                 self.counters["generated_tokens"] += 1
                 if done:
                     self.scheduler.finish(req)
+                    self.runner.adapter_of.pop(req.rid, None)
                 out.append((req.rid, int(tok), done))
         return out
 
@@ -217,14 +273,21 @@ class Engine:
             self.runner.prepare_decode(rids)
         return queue
 
-    def generate(self, prompts: Sequence[Sequence[int]], params: Union[SamplingParams, Sequence[SamplingParams], None] = None
-                 ) -> List[List[int]]:
-        """Generate for every prompt (token ids in, token ids out); continuous batching inside."""
+    def generate(self, prompts: Sequence[Sequence[int]], params: Union[SamplingParams, Sequence[SamplingParams], None] = None,
+                 adapters: Union[str, Sequence[Optional[str]], None] = None) -> List[List[int]]:
+        """Generate for every prompt (token ids in, token ids out); continuous batching inside.  ``adapters``: a loaded adapter's name
+        for all prompts, or one (or None) for each."""
         if params is None or isinstance(params, SamplingParams):
             params = [params or SamplingParams()] * len(prompts)
         if len(params) != len(prompts):
             raise ValueError("one SamplingParams per prompt")
-        rids = [self.add_request(p, sp) for p, sp in zip(prompts, params)]
+        names = [adapters] * len(prompts) if adapters is None or isinstance(adapters, str) else list(adapters)
+        if len(names) != len(prompts):
+            raise ValueError("one adapter name (or None) per prompt")
+        for name in names:
+            if name is not None and name not in self._adapters:
+                raise ValueError(f"adapter {name!r} is not loaded (loaded: {sorted(self._adapters)})")
+        rids = [self.add_request(p, sp, adapter=a) for p, sp, a in zip(prompts, params, names)]
         while self.has_unfinished():
             self.step()
         return [list(self._requests[r].output) for r in rids]
@@ -264,6 +327,7 @@ class Engine:
     def abort(self, rid: Hashable, reason: str = "aborted") -> None:
         """End a request now, wherever it stands; its pages and state slot are free at once."""
         self.scheduler.abort(self._requests[rid], reason)
+        self.runner.adapter_of.pop(rid, None)
 
     def sample_from_logits(self, logits: torch.Tensor, params: Optional[SamplingParams] = None, draw_index: int = 0,
                            prompt_tokens: Sequence[int] = (), output_tokens: Sequence[int] = ()) -> int:

@@ -116,6 +116,21 @@ class CausalLM:
         self.final_norm.load_weights(get)
         self.lm_head.load_weights(get, self.embedding)
 
+    # ---- adapters ------------------------------------------------------
+    def enable_adapters(self, slots: int, rank: int) -> Dict[str, tuple]:
+        """Make room for ``slots`` low-rank adapters of up to ``rank`` beside every projection that takes them (parts/adapters.py).
+        Returns checkpoint tensor name -> (part, product, which of its stacked matrices)."""
+        targets: Dict[str, tuple] = {}
+        for layer in self.layers:
+            if not getattr(layer, "takes_adapters", False):
+                continue
+            for part in layer.parts():
+                names = part.adapter_targets() if hasattr(part, "adapter_targets") else {}
+                if names:
+                    part.enable_adapters(slots, rank)
+                    targets.update({name: (part,) + where for name, where in names.items()})
+        return targets
+
     def weight_bytes(self, include_embedding: bool = True) -> int:
         seen, total = set(), 0
 

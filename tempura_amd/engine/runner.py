@@ -46,6 +46,8 @@ class StepContext:
     logit_rows[m]     flattened token indices whose logits are returned
     Host copies (``q_starts``, ``q_lens``, ``ctx_lens``, ``state_slot_list``) serve parts
     that loop over requests on the host.
+    ``adapter_ids`` (int32 [n], or None): the adapter slot of each token's request, -1 without one; None: no
+    request of the step has an adapter.
     ``shared``: what the parts of several layers compute once per step and keep under a key of
     their own (a rotation table, for instance); empty when the step begins.
     """
@@ -69,6 +71,7 @@ class StepContext:
         self.q_lens: List[int] = []
         self.ctx_lens: List[int] = []
         self.state_slot_list: List[int] = []
+        self.adapter_ids = None
         self.shared: dict = {}
 
 
@@ -81,13 +84,14 @@ class _DecodeGraph:
     graphs are keyed by batch size with all per-step values device-read in the same way
     (/root/reference/engine/src/cutile_gpu_forward.rs:939-953)."""
 
-    def __init__(self, runner: "ModelRunner", rows: int, ctx_bound: int):
+    def __init__(self, runner: "ModelRunner", rows: int, ctx_bound: int, adapters: bool = False):
         self.rows = rows
+        self.adapters = adapters       # (the step's adapter slots lie behind everything else)
         self.ctx_bound = ctx_bound
         self.width = (ctx_bound + runner.page_size - 1) // runner.page_size
         n_groups = len(runner.cache.groups)
         # layout: tokens, positions, context_lens, state_slots | per group: table, slots
-        self.sizes = [rows, rows, rows, rows] + [rows * self.width] * n_groups + [rows] * n_groups
+        self.sizes = [rows, rows, rows, rows] + [rows * self.width] * n_groups + [rows] * n_groups + [rows] * adapters
         self.offs = np.cumsum([0] + self.sizes)
         total = int(self.offs[-1])
         # two pinned buffers taken in turn (the next step may be staged while the last copy is still queued),
@@ -119,6 +123,8 @@ class _DecodeGraph:
         ctx.logit_rows = None                     # every row
         ctx.block_tables = [self.view(4 + g).view(self.rows, self.width) for g in range(n_groups)]
         ctx.slot_mapping = [self.view(4 + n_groups + g) for g in range(n_groups)]
+        if self.adapters:
+            ctx.adapter_ids = self.view(4 + 2 * n_groups)
         ctx.max_q_len = 1
         ctx.num_single = self.rows
         ctx.max_context_len = self.width * runner.page_size
@@ -184,6 +190,9 @@ class ModelRunner:
         self.steps_run = 0
         self.tokens_run = 0
         self._staging = _PackedStaging(self.device)
+        self._adapter_staging = _PackedStaging(self.device)
+        #: requests with an adapter -> its slot (whoever adds a request says so here, for as long as it runs)
+        self.adapter_of: Dict[Hashable, int] = {}
         #: host time spent packing the inputs of eager steps, and how many such steps there were
         self.host_seconds = {"pack": 0.0}
         self.host_steps = {"pack": 0}
@@ -309,12 +318,19 @@ class ModelRunner:
         ctx.q_lens = n_new.tolist()
         ctx.ctx_lens = ctx_lens.tolist()
         ctx.state_slot_list = slots
+        if self._adapted(e.rid for e in entries):
+            ids = np.repeat(np.asarray([self.adapter_of.get(e.rid, -1) for e in entries], dtype=np.int32), n_new)
+            self._adapter_staging.take(N)[:N] = ids
+            ctx.adapter_ids = self._adapter_staging.send(N)
         self.host_seconds["pack"] += time.perf_counter() - t_start
         self.host_steps["pack"] += 1
         return tok_dev, ctx
 
+    def _adapted(self, rids) -> bool:
+        return bool(self.adapter_of) and any(rid in self.adapter_of for rid in rids)
+
     # ---- decode steps as a graph -----------------------------------------
-    def _graph_for(self, rows: int, ctx_len: int) -> Optional[_DecodeGraph]:
+    def _graph_for(self, rows: int, ctx_len: int, adapters: bool = False) -> Optional[_DecodeGraph]:
         # rows padded to a power of two, beyond 128 to a multiple of 128: the products see as many blocks of rows as
         # in the unpadded step and so choose the same tiles and parts of K (the same bits as an eager step)
         bucket = ops.decode_rows_padded(rows)
@@ -322,10 +338,10 @@ class ModelRunner:
         while bound < ctx_len:
             bound *= 2
         bound = min(bound, (self.model.spec.max_positions + self.page_size - 1) // self.page_size * self.page_size)
-        key = (bucket, bound)
+        key = (bucket, bound, True) if adapters else (bucket, bound)
         g = self._graphs.get(key)
         if g is None:
-            g = _DecodeGraph(self, bucket, bound)
+            g = _DecodeGraph(self, bucket, bound, adapters)
             self._graphs[key] = g
         return g
 
@@ -335,6 +351,10 @@ class ModelRunner:
         g.copied[i].synchronize()                  # the last copy out of this pinned buffer has finished
         self.cache.fill_decode(rids, tokens, g.rows, g.width,
                                [self.pools.scratch_page(gi) for gi in range(len(self.cache.groups))], g.host_nps[i])
+        if g.adapters:
+            ids = g.host_nps[i][int(g.offs[-2]):]
+            ids[:] = -1
+            ids[: len(rids)] = [self.adapter_of.get(r, -1) for r in rids]
         g.packed.copy_(g.hosts[i], non_blocking=True)
         g.copied[i].record()
 
@@ -355,7 +375,7 @@ class ModelRunner:
             self.cache.reserve_many(rids, [1] * len(rids))
         except PagesExhausted:
             return False
-        g = self._graph_for(len(rids), ctx_len)
+        g = self._graph_for(len(rids), ctx_len, self._adapted(rids))
         if g.graph is None:
             return False
         self._fill_graph_inputs(g, rids, [0] * len(rids))
@@ -380,7 +400,7 @@ class ModelRunner:
                 g.tok_copied.record()
         else:
             ctx_len = self.cache.max_num_tokens(rids) + 1
-            g = self._graph_for(n, ctx_len)
+            g = self._graph_for(n, ctx_len, self._adapted(rids))
             self._fill_graph_inputs(g, rids, [0] * n if on_device else tokens)
         if on_device:
             g.packed[:n].copy_(tokens)

@@ -906,7 +906,8 @@ class Adapters:
     of 8 are padded with zeros here, once; otherwise the tensors are kept as they are, and what is written into them later counts."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, ends=None, interleaved: bool = False):
-        _dev_ok(a, b, scales)
+        if _backend is None:
+            _dev_ok(a, b, scales)
         _need(a.dim() == b.dim() == 3 and a.dtype == b.dtype and a.dtype in (torch.bfloat16, torch.float32),
               "Adapters: a [slots, slices * rank, k] and b [slots, n, rank], bfloat16 or float32")
         self.slots, self.n, rank = b.shape
@@ -959,7 +960,9 @@ def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, re
     # rows of 4,096 x 4,096 and nothing for 731 of 8,192 x 2,048, where the other order reads it in a pass of its own, 17 us)
     y = torch.empty((m, adapters.n), dtype=torch.float32, device=x.device) if residual is None else residual
     ranks = adapters.slices * adapters.rank
-    parts = max(1, min(8, k // 512, 256 // (-(-m // 64) * -(-ranks // 64))))
+    # (single tokens by the rows that a captured step of as many has: the order of a row's sums hangs on the parts of K)
+    windows = -(-(decode_rows_padded(m) if max_run == 1 else m) // 64)
+    parts = max(1, min(8, k // 512, 256 // (windows * -(-ranks // 64))))
     _adapter_add(x, adapters, ids, y, parts, int(residual is None))
     return linear(x, w, torch.float32, residual=y)
 

@@ -45,6 +45,7 @@ from dataclasses import dataclass
 import torch
 
 from ..kernels import ops
+from .adapters import TakesAdapters
 from .base import BranchMixer, CacheSpec, Mixer, WeightInfo, build_part, pad_rows, part_class, register_part
 from .rope import paired_order, reorder_heads
 
@@ -71,7 +72,7 @@ def distance_table(rows: torch.Tensor, max_distance: int, window) -> torch.Tenso
     return rows.to(torch.float32)[index].t().contiguous()
 
 
-class PagedAttention(Mixer):
+class PagedAttention(TakesAdapters, Mixer):
     graph_safe = True      # only kernels on device-resident step data: may be captured in a graph
     #: the value cache is transposed, eight consecutive tokens of one element being one 16-byte piece: a portion that
     #: starts at a multiple of eight positions (and of eight rows of the batch) has its values stored piece by piece
@@ -251,6 +252,21 @@ class PagedAttention(Mixer):
             self.sink_w = self._to_device(get(w["sink"]), torch.float32)
         self.position.load_weights(get)
 
+    # ---- adapters: beside q, k, v and o of an attention whose rows pass no kernel but rotation and cache write -------------
+    def _plain(self) -> bool:
+        return self.position.rotary() is not None and not (self.plain_qk or self.extended or self.gate or self.side_rows is not None)
+
+    def adapter_targets(self):
+        w = self.spec.weights
+        return {w["q"]: ("qkv", 0), w["k"]: ("qkv", 1), w["v"]: ("qkv", 2), w["o"]: ("o", 0)} if self._plain() else {}
+
+    def adapter_products(self):
+        return {"qkv": {"k": self.hidden_size, "rows": [self.q_dim, self.kv_dim, self.v_dim]}, "o": {"k": self.q_dim, "rows": [self.hidden_size]}}
+
+    def adapter_rows(self, name, b):
+        w = self.spec.weights
+        return self._paired(b) if name in (w["q"], w["k"]) else b
+
     def cache_spec(self):
         kind, span = ("window", self.window) if self.window is not None else ("chunk", self.chunk) if self.chunk else ("full", None)
         if self.keep_first:
@@ -261,13 +277,14 @@ class PagedAttention(Mixer):
 
     def forward(self, x, ctx, cache, residual, next_norm=None):
         rot = self.position.rotary()
+        ids = self.adapters_of(ctx)
         q = None
         gates = None       # float32 rows that hold the gate's and the side rows' columns
         if self.rows_path:
             q, gates = self._project_rows(x, ctx, cache, rot)
         elif self.plain_qk:
             q = self._project_plain(x, ctx, cache)
-        elif rot is not None and cache.writes and not self.extended:
+        elif rot is not None and cache.writes and not self.extended and ids is None:
             rows = x.x if isinstance(x, ops.Prenormed) else x
             if ops.linear_rope_ok(x.shape[0], self.wqkv.shape[0], x.shape[1], self.head_dim, rot[1], cache.k.shape[2],
                                   rows.dtype, cache.k.dtype, isinstance(x, ops.Prenormed)):
@@ -286,7 +303,7 @@ class PagedAttention(Mixer):
         step = {**into, "shared": shared}
         a, attended = None, False
         if q is None:
-            rows = self._project(x, cache, rot)
+            rows = self._project(x, cache, rot) if ids is None else self._project_adapted(x, ids, ctx, cache)
             if cache.writes and (rot is not None or type(self.position).__name__ == "NoPosition") and not self.softcap and self.dist_table is None \
                     and ops.attention_rows_ok(rows, ctx, self.num_heads, self.num_kv_heads, self.head_dim, self.value_dim, cache.k) \
                     and ops.attention_rows_pays(ctx, self.num_kv_heads, self.head_dim, int(self.window or 0), self.keep_first, self.chunk):
@@ -326,6 +343,9 @@ class PagedAttention(Mixer):
             if residual is not None:
                 raise ValueError("attention: with side rows the output comes back, it is not added")
             return ops.linear(a, self.wo, torch.float32), (gates, self.side_col0)
+        if ids is not None:
+            y = self.product(a, self.wo, "o", ids, ctx, residual)
+            return y if residual is None else None
         if residual is None or isinstance(residual, ops.StreamClose):
             return ops.linear(a, self.wo, torch.float32, residual=residual)
         if next_norm is None:
@@ -365,6 +385,11 @@ class PagedAttention(Mixer):
             raise ValueError("attention: qk_norm, value_dim, sink and keep_first need a rotary position part or none")
         w = self.wqkv if cache.writes else ops.weight_rows(self.wqkv, 0, self.q_dim)
         return ops.linear(x, w, torch.float32, partial_ok=rot is not None and not self.extended)
+
+    def _project_adapted(self, x, ids, ctx, cache):
+        """The projection's rows with the adapters' share (of a call that reads another call's cache q alone)."""
+        rows = self.product(x, self.wqkv, "qkv", ids, ctx)
+        return rows if cache.writes else rows[:, : self.q_dim].contiguous()
 
     def _rotate(self, qkv, ctx, cache, rot):
         """q (rotated, [n, heads, head_dim]) of the projection's rows; k and v go to the cache.  With a norm per head the rows are

@@ -28,6 +28,8 @@ class ArrangedBlock:
     ROLES: dict = {}
     #: roles a layer may leave out (the attribute is then None)
     OPTIONAL: frozenset = frozenset()
+    #: True: parts of this arrangement may have low-rank adapters beside their projections (parts/adapters.py)
+    takes_adapters = False
     #: what this arrangement hands to the block behind it (blocks of the same kind only): see ``entry_norm``
     handoff = None
 
@@ -67,6 +69,7 @@ class ArrangedBlock:
 class PreNormBlock(ArrangedBlock):
     ROLES = {"mixer_norm": "norm", "mixer": "mixer", "ffn_norm": "norm", "ffn": "ffn"}
     handoff = "split_norm"
+    takes_adapters = True      # its parts get plain normed rows when they do not say ``split_norm``
 
     def entry_norm(self, m):
         """What the part before this block needs to prepare this block's first norm for ``m`` rows, or None."""

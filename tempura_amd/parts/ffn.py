@@ -7,10 +7,11 @@ from __future__ import annotations
 import torch
 
 from ..kernels import ops
+from .adapters import TakesAdapters
 from .base import FeedForward, WeightInfo, register_part
 
 
-class SwiGLU(FeedForward):
+class SwiGLU(TakesAdapters, FeedForward):
     graph_safe = True      # only kernels on device-resident step data: may be captured in a graph
     split_norm = True      # takes rows whose norm its first product finishes; prepares the next norm in its last
 
@@ -41,7 +42,22 @@ class SwiGLU(FeedForward):
             self.w13 = ops.tile_weight(torch.cat([gate, up], dim=0).contiguous())
         self.w2 = ops.tile_weight(self._to_device(get(w["down"])))
 
+    def adapter_targets(self):
+        w = self.spec.weights
+        return {w["gate"]: ("w13", 0), w["up"]: ("w13", 1), w["down"]: ("w2", 0)}
+
+    def adapter_products(self):
+        i = self.intermediate_size
+        return {"w13": {"k": self.hidden_size, "rows": [i, i], "interleaved": self.fused}, "w2": {"k": i, "rows": [self.hidden_size]}}
+
     def forward(self, x, ctx, residual, next_norm=None):
+        ids = self.adapters_of(ctx)
+        if ids is not None:
+            # (the adapters' share comes in front of the activation, which is then a kernel of its own)
+            gu = self.product(x, self.w13, "w13", ids, ctx)
+            a = ops.gated_act(gu, self.dtype, interleaved=True) if self.fused else ops.swiglu(gu, self.dtype)
+            self.product(a, self.w2, "w2", ids, ctx, residual)
+            return None
         if self.fused:
             # (a few rows go to the next product k-blocked: it reads them straight from global memory)
             a = ops.linear_swiglu(x, self.w13, blocked_out=True)
