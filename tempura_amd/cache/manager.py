@@ -81,6 +81,7 @@ class CacheManager:
             raise ValueError(native.last_error())
         self.pools = [_PoolView(self, g, int(n)) for g, n in enumerate(num_pages)]
         self._slot_of: Dict[Hashable, int] = {}
+        self._shared: Dict[Hashable, tuple] = {}     # request -> (mark, tokens) that it began with
         #: bumped by everything that changes what a request holds or where its next token goes (add, release,
         #: commit, truncate): whoever keeps values derived from the tables compares it before using them
         self.generation = 0
@@ -118,11 +119,32 @@ class CacheManager:
     def release(self, rid) -> None:
         """The request has ended: every page and its state slot go back."""
         s = self._slot_of.pop(rid, None)
+        self._shared.pop(rid, None)
         if s is None:
             raise ValueError(f"request {rid!r} is not live (released twice?)")
         self.generation += 1
         if self._lib.cc_release(self._h, s) != 0:
             raise RuntimeError(native.last_error())
+
+    @property
+    def shareable(self) -> bool:
+        """Whether requests may begin with pages of another: no group ever gives pages back."""
+        return bool(self.groups) and all(s.kind == "full" for s in self.groups)
+
+    def share(self, rid, donor, num_tokens: int) -> None:
+        """The fresh request ``rid`` begins with the first ``num_tokens`` tokens (whole pages) of ``donor``, whose pages it shares; they are held
+        until the last request that has them ends."""
+        if not self.shareable:
+            raise ValueError("pages can be shared only where every group keeps all keys")
+        if self._lib.cc_share(self._h, self._slot(rid), self._slot(donor), int(num_tokens)) != 0:
+            raise ValueError(native.last_error())
+        # (the last shared page marks what is shared: a page is in another table only together with all pages in front of it)
+        self._shared[rid] = (self.table(rid, 0)[-1], int(num_tokens))
+        self.generation += 1
+
+    def shared(self, rid):
+        """(mark, tokens) that ``rid`` began with, or None; the mark is the same for live requests that began with the same pages."""
+        return self._shared.get(rid)
 
     def num_tokens(self, rid) -> int:
         return self._lib.cc_num_tokens(self._h, self._slot(rid))
@@ -177,6 +199,8 @@ class CacheManager:
         self.generation += 1
         if self._lib.cc_truncate(self._h, self._slot(rid), int(num_tokens)) != 0:
             raise ValueError(native.last_error())
+        if rid in self._shared and num_tokens < self._shared[rid][1]:
+            del self._shared[rid]
 
     def table(self, rid, g: int) -> List[int]:
         s = self._slot(rid)

@@ -39,7 +39,7 @@ int fail(const char* fmt, ...) {
 struct Pool {
   int num_pages = 0;
   std::vector<int> free_list;  // LIFO: the most recently freed page is handed out first
-  std::vector<uint8_t> held;
+  std::vector<int> held;       // in how many tables a page is (requests that begin with the same tokens may share their first pages)
 
   explicit Pool(int n) : num_pages(n), held(n, 0) {
     free_list.reserve(n);
@@ -55,8 +55,7 @@ struct Pool {
   int release(int p) {
     if (p < 0 || p >= num_pages) return fail("page %d out of range", p);
     if (!held[p]) return fail("page %d freed twice (or never allocated)", p);
-    held[p] = 0;
-    free_list.push_back(p);
+    if (--held[p] == 0) free_list.push_back(p);
     return 0;
   }
   // every page is either free or held, exactly once
@@ -69,7 +68,7 @@ struct Pool {
       on_list[p] = 1;
     }
     int n_held = 0;
-    for (int p = 0; p < num_pages; ++p) n_held += held[p];
+    for (int p = 0; p < num_pages; ++p) n_held += held[p] > 0;
     if (n_held + (int)free_list.size() != num_pages) return fail("a page was lost");
     return 0;
   }
@@ -78,6 +77,7 @@ struct Pool {
 struct Request {
   bool live = false;
   int num_tokens = 0;                      // tokens whose keys and values are in the cache
+  int shared_tokens = 0;                   // of them, those in pages that another request wrote (whole pages)
   std::vector<std::vector<int>> tables;    // per group: logical page -> physical page, -1 = none
   std::vector<int> first_live;             // per group: first logical page still held
 };
@@ -206,10 +206,35 @@ int cc_add(void* h) {
   c->free_state.pop_back();
   Request& r = c->reqs[s];
   r.live = true;
-  r.num_tokens = 0;
+  r.num_tokens = r.shared_tokens = 0;
   r.tables.assign(c->n_groups(), {});
   r.first_live.assign(c->n_groups(), 0);
   return s;
+}
+
+// A fresh request begins with the first num_tokens tokens of `donor`, whose pages (whole ones, of groups that keep every key) it shares; they go back
+// when the last request that has them ends.  Nothing is ever written into them: a request writes behind its last token.
+int cc_share(void* h, int req, int donor, int num_tokens) {
+  Core* c = (Core*)h;
+  Request *r = c->live(req), *d = c->live(donor);
+  if (!r || !d) return -1;
+  if (req == donor) return fail("a request cannot share its own pages");
+  if (r->num_tokens != 0) return fail("only a request without tokens can begin with another's");
+  for (const std::vector<int>& t : r->tables)
+    if (!t.empty()) return fail("only a request without pages can begin with another's");
+  if (num_tokens <= 0 || num_tokens % c->page_size != 0) return fail("shared tokens must fill whole pages of %d", c->page_size);
+  if (num_tokens > d->num_tokens) return fail("%d tokens to share, the donor has %d", num_tokens, d->num_tokens);
+  for (int g = 0; g < c->n_groups(); ++g)
+    if (c->first_needed(g, num_tokens) > 0 || c->first_needed(g, 0x3fffffff) > 0) return fail("group %d gives pages back: they cannot be shared", g);
+  const int pages = num_tokens / c->page_size;
+  for (int g = 0; g < c->n_groups(); ++g)
+    for (int lp = 0; lp < pages; ++lp) {
+      const int p = d->tables[g][lp];
+      r->tables[g].push_back(p);
+      ++c->pools[g].held[p];
+    }
+  r->num_tokens = r->shared_tokens = num_tokens;
+  return 0;
 }
 
 // The request has ended: every page and its state slot go back.
@@ -295,6 +320,14 @@ int cc_truncate(void* h, int req, int num_tokens) {
   for (int g = 0; g < c->n_groups(); ++g)
     if (num_tokens < r->num_tokens && c->first_needed(g, num_tokens) < r->first_live[g])
       return fail("group %d has given back pages that the truncated request would need", g);
+  // the page that the next token would be written into must be this request's alone
+  if (num_tokens < r->num_tokens && num_tokens % c->page_size != 0)
+    for (int g = 0; g < c->n_groups(); ++g) {
+      const int lp = num_tokens / c->page_size;
+      if (lp < (int)r->tables[g].size() && r->tables[g][lp] >= 0 && c->pools[g].held[r->tables[g][lp]] > 1)
+        return fail("group %d: the page of position %d is shared with another request", g, num_tokens);
+    }
+  r->shared_tokens = std::min(r->shared_tokens, num_tokens);
   const int keep = (num_tokens + c->page_size - 1) / c->page_size;
   for (int g = 0; g < c->n_groups(); ++g) {
     std::vector<int>& table = r->tables[g];
@@ -349,7 +382,7 @@ double cc_waste_ratio(void* h) {
   if (held == 0) return 0.0;
   for (const Request& r : c->reqs)
     if (r.live)
-      for (int g = 0; g < c->n_groups(); ++g) used += std::max(0, r.num_tokens - r.first_live[g] * c->page_size);
+      for (int g = 0; g < c->n_groups(); ++g) used += std::max(0, r.num_tokens - r.shared_tokens - r.first_live[g] * c->page_size);
   return std::max(0.0, 1.0 - (double)used / (double)held);
 }
 
@@ -359,19 +392,20 @@ int cc_check(void* h) {
   for (int g = 0; g < c->n_groups(); ++g) {
     const Pool& pool = c->pools[g];
     if (pool.check() != 0) return -1;
-    std::vector<uint8_t> seen(pool.num_pages, 0);
+    std::vector<int> seen(pool.num_pages, 0);
     int n_seen = 0;
     for (const Request& r : c->reqs) {
       if (!r.live) continue;
       for (int p : r.tables[g]) {
         if (p < 0) continue;
         if (p >= pool.num_pages) return fail("group %d: page %d out of range", g, p);
-        if (seen[p]) return fail("group %d: page %d is in two tables", g, p);
+        if (seen[p] >= std::max(1, pool.held[p])) return fail("group %d: page %d is in two tables", g, p);
         if (!pool.held[p]) return fail("group %d: page %d is in a table but free", g, p);
-        seen[p] = 1;
-        ++n_seen;
+        n_seen += seen[p]++ == 0;
       }
     }
+    for (int p = 0; p < pool.num_pages; ++p)
+      if (seen[p] != 0 && seen[p] != pool.held[p]) return fail("group %d: page %d is in %d tables and held for %d", g, p, seen[p], pool.held[p]);
     const int held = pool.num_pages - pool.num_free();
     if (n_seen != held) return fail("group %d: %d pages held by no request", g, held - n_seen);
   }

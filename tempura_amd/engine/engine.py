@@ -32,7 +32,7 @@ class Engine:
                  max_seq_len: Optional[int] = None, max_num_batched_tokens: int = 2048,
                  prefill_chunk_size: int = 512, device: str = "cuda:0", use_graph: bool = True,
                  chain_steps: bool = True, fill_budget: bool = True, admit_headroom: Optional[float] = 0.02,
-                 max_adapters: int = 0, max_adapter_rank: int = 16):
+                 max_adapters: int = 0, max_adapter_rank: int = 16, max_prefixes: int = 0):
         """``model``: a folder with config.json and safetensors, or (with ``random_weights``) a typed
         configuration such as ``LlamaConfig``/``PRESETS[name]``.
         ``kv_pages``: cache pages per group; by default as many as ``gpu_memory_utilization`` of the
@@ -47,7 +47,8 @@ class Engine:
         ``admit_headroom``: share of the cache pages that an admission leaves free beside running requests (None:
         a request comes in as soon as its first portion fits; see ``SchedulerConfig.admit_headroom``).
         ``max_adapters``: how many low-rank adapters of up to ``max_adapter_rank`` may be loaded at a time (``load_adapter``); the room for
-        them is taken at once, and the model's norms run as kernels of their own (0: neither)."""
+        them is taken at once, and the model's norms run as kernels of their own (0: neither).
+        ``max_prefixes``: how many prefixes may be held at a time for requests to begin with (``hold_prefix``)."""
         self.device = torch.device(device)
         if isinstance(model, str):
             if random_weights:
@@ -71,10 +72,10 @@ class Engine:
         self.max_seq_len = min(int(max_seq_len or spec.max_positions), spec.max_positions)
         self.page_size = int(page_size)
         if kv_pages is None:
-            kv_pages = self._pages_from_memory(gpu_memory_utilization, max_batch_size)
+            kv_pages = self._pages_from_memory(gpu_memory_utilization, max_batch_size + max(0, max_prefixes))
         # (one request slot more than the scheduler hands out: ``forward`` and ``dump`` run their fresh request in it
         # also while ``max_batch_size`` requests are live)
-        self.runner = ModelRunner(self.model, self.page_size, int(kv_pages), max_requests=max_batch_size + 1,
+        self.runner = ModelRunner(self.model, self.page_size, int(kv_pages), max_requests=max_batch_size + 1 + int(max_prefixes),
                                   use_graph=use_graph)
         self.scheduler = Scheduler(
             SchedulerConfig(max_num_seqs=max_batch_size, max_num_batched_tokens=max_num_batched_tokens,
@@ -83,6 +84,11 @@ class Engine:
                             portion_align=self.model.portion_align()),
             self.runner.cache)
         self.sampler = Sampler(spec.vocab_size, self.device, default_seed=seed)
+        if max_prefixes < 0 or (max_prefixes and not self.runner.can_share):
+            raise ValueError("max_prefixes must not be negative, and only a model whose layers all keep every key, and nothing else of what came "
+                             "before, lets requests begin with the pages of another")
+        self.max_prefixes = int(max_prefixes)
+        self._prefixes: Dict[int, Tuple[Hashable, List[int], int, Optional[str]]] = {}      # handle -> request, tokens, shared tokens, adapter
         self._ids = itertools.count()            # request ids that add_request hands out: 0, 1, 2, ...
         self._own_ids = itertools.count()        # names of the engine's own short-lived requests (forward, profile)
         self._requests: Dict[Hashable, Request] = {}
@@ -146,13 +152,69 @@ class Engine:
         busy = [rid for rid, req in self._requests.items() if req.state != RequestState.FINISHED and self.runner.adapter_of.get(rid) == slot]
         if busy:
             raise ValueError(f"adapter {name!r} is in use by request {busy[0]!r}")
+        if any(p[3] == name for p in self._prefixes.values()):
+            raise ValueError(f"adapter {name!r} is in use by a prefix that is held")
         self._free_adapters.append(self._adapters.pop(name))
+
+    # ---- prefixes ------------------------------------------------------------
+    def hold_prefix(self, token_ids: Sequence[int], adapter: Optional[str] = None) -> int:
+        """Compute the keys and values of tokens that many requests will begin with (a system prompt, a document) and hold them; the handle
+        goes to ``add_request``.  Requests share its whole pages, compute only what comes behind them, and in a step with several of them
+        attention reads the shared keys once (``ops.prefix_attention``).  ``adapter``: the adapter that it is computed with, and that such
+        requests then have to name."""
+        tokens = [int(t) for t in token_ids]
+        if len(self._prefixes) >= self.max_prefixes:
+            raise ValueError(f"{len(self._prefixes)} prefixes are held, there is room for no more (max_prefixes)")
+        if any(t < 0 or t >= self.model.spec.vocab_size for t in tokens):
+            raise ValueError(f"a token id outside the vocabulary of {self.model.spec.vocab_size}")
+        if adapter is not None and adapter not in self._adapters:
+            raise ValueError(f"adapter {adapter!r} is not loaded (loaded: {sorted(self._adapters)})")
+        shared = len(tokens) // self.page_size * self.page_size
+        if shared == 0 or len(tokens) + 1 >= self.scheduler.config.max_model_len:
+            raise ValueError(f"a prefix of {len(tokens)} tokens: at least a page ({self.page_size}), and fewer than a request may have")
+        pages = shared // self.page_size
+        unfinished = [r.pages for r in self._requests.values() if r.state != RequestState.FINISHED]
+        free = min(p.num_pages for p in self.runner.cache.pools) - self.scheduler.pages_kept - pages
+        if free < max(unfinished, default=1):
+            raise ValueError(f"a prefix of {pages} pages leaves {free} pages a group, too few for the requests")
+        if self._ahead is not None:      # a queued step's logits live in a graph's output buffer: keep a copy
+            self._ahead = (self._ahead[0], ops.take_rows(self._ahead[1]))
+        handle = next(self._own_ids)
+        rid = ("prefix", handle)
+        self.runner.add_request(rid)
+        if adapter is not None:
+            self.runner.adapter_of[rid] = self._adapters[adapter]
+        try:
+            budget = self.scheduler.config.max_num_batched_tokens
+            for at in range(0, shared, budget):
+                self.runner.step([StepEntry(rid, tokens[at: min(shared, at + budget)], [])])
+        except BaseException:
+            self.runner.end_request(rid)
+            self.runner.adapter_of.pop(rid, None)
+            raise
+        self._prefixes[handle] = (rid, tokens, shared, adapter)
+        self.scheduler.pages_kept += pages
+        return handle
+
+    def release_prefix(self, handle: int) -> None:
+        """Hold a prefix no longer; requests that began with it keep its pages until they end."""
+        if handle not in self._prefixes:
+            raise KeyError(f"prefix {handle!r} is not held")
+        rid, _, shared, _ = self._prefixes.pop(handle)
+        for req in self._requests.values():      # (one that has to be computed again then needs these pages too)
+            if req.state != RequestState.FINISHED and req.prefix is not None and req.prefix[0] == rid:
+                req.pages += shared // self.page_size
+        self.runner.end_request(rid)
+        self.runner.adapter_of.pop(rid, None)
+        self.scheduler.pages_kept -= shared // self.page_size
 
     # ---- requests ------------------------------------------------------------
     def add_request(self, prompt_ids: Sequence[int], params: Optional[SamplingParams] = None,
-                    rid: Optional[Hashable] = None, logprobs_top_n: Optional[int] = None, adapter: Optional[str] = None) -> Hashable:
+                    rid: Optional[Hashable] = None, logprobs_top_n: Optional[int] = None, adapter: Optional[str] = None,
+                    prefix: Optional[int] = None) -> Hashable:
         """Queue a request.  With ``logprobs_top_n`` (0..20) every generated token gets a ``TokenLogprob``
-        record in ``request(rid).logprobs``.  ``adapter``: the name of a loaded adapter (``load_adapter``)."""
+        record in ``request(rid).logprobs``.  ``adapter``: the name of a loaded adapter (``load_adapter``).  ``prefix``: a handle of
+        ``hold_prefix``; the request's prompt is that prefix followed by ``prompt_ids`` (at least one token)."""
         params = params or SamplingParams()
         if rid is None:
             rid = next(self._ids)
@@ -160,13 +222,23 @@ class Engine:
             raise ValueError(f"request id {rid!r} is in use")
         if adapter is not None and adapter not in self._adapters:
             raise ValueError(f"adapter {adapter!r} is not loaded (loaded: {sorted(self._adapters)})")
+        begins = None
+        if prefix is not None:
+            if prefix not in self._prefixes:
+                raise ValueError(f"prefix {prefix!r} is not held")
+            began, tokens, shared, named = self._prefixes[prefix]
+            if named != adapter:
+                raise ValueError(f"prefix {prefix!r} was computed with adapter {named!r}, the request names {adapter!r}")
+            if len(prompt_ids) == 0:
+                raise ValueError("a request needs at least one token behind its prefix")
+            prompt_ids, begins = tokens + list(prompt_ids), (began, shared)
         vocab = self.model.spec.vocab_size
         for t in prompt_ids:
             if t < 0 or t >= vocab:
                 raise ValueError(f"token id {t} outside the vocabulary of {vocab}")
         eos = params.eos_token_id if params.eos_token_id is not None else self.model.spec.eos_token_ids
         req = Request(rid, [int(t) for t in prompt_ids], params, tuple(int(e) for e in eos),
-                      logprobs_top_n=logprobs_top_n)
+                      logprobs_top_n=logprobs_top_n, prefix=begins)
         self.scheduler.add_request(req)
         self._requests[rid] = req
         self.runner.adapter_of.pop(rid, None)
@@ -207,7 +279,14 @@ class Engine:
             # (and portions whose length is no such multiple, the ends of prompts, go behind the others: every
             # portion behind one of them starts at an odd row)
             align = self.scheduler.config.portion_align
-            items.sort(key=lambda it: (it.count == 1, it.count % align != 0 if it.count > 1 else -it.start))
+            # Requests that begin with the same pages are neighbours among their like (-1: none), for attention to read those once.
+            began = self.runner.cache.shared
+
+            def place(it):
+                with_prefix = began(it.request.rid)
+                group = -1 if with_prefix is None else with_prefix[0]
+                return (it.count == 1, it.count % align != 0 if it.count > 1 else False, group, -it.start if it.count == 1 else 0)
+            items.sort(key=place)
             entries = []
             for it in items:
                 toks = it.request.step_tokens(it.start, it.count)

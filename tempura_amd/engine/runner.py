@@ -48,6 +48,8 @@ class StepContext:
     that loop over requests on the host.
     ``adapter_ids`` (int32 [n], or None): the adapter slot of each token's request, -1 without one; None: no
     request of the step has an adapter.
+    ``shared_keys`` (``ops.SharedKeys``, or None): which neighbouring requests begin with the same keys, where it pays to read
+    them once; ``max_own_len``: the most keys a request has behind them.
     ``shared``: what the parts of several layers compute once per step and keep under a key of
     their own (a rotation table, for instance); empty when the step begins.
     """
@@ -72,6 +74,8 @@ class StepContext:
         self.ctx_lens: List[int] = []
         self.state_slot_list: List[int] = []
         self.adapter_ids = None
+        self.shared_keys = None
+        self.max_own_len = 0
         self.shared: dict = {}
 
 
@@ -84,14 +88,19 @@ class _DecodeGraph:
     graphs are keyed by batch size with all per-step values device-read in the same way
     (/root/reference/engine/src/cutile_gpu_forward.rs:939-953)."""
 
-    def __init__(self, runner: "ModelRunner", rows: int, ctx_bound: int, adapters: bool = False):
+    #: runs of requests that a captured step has room for, eight of which may share keys
+    RUNS = 17
+
+    def __init__(self, runner: "ModelRunner", rows: int, ctx_bound: int, adapters: bool = False, shared: Optional[tuple] = None):
         self.rows = rows
         self.adapters = adapters       # (the step's adapter slots lie behind everything else)
+        self.shared = shared           # (bounds on shared and own keys; the runs lie in front of the adapter slots)
         self.ctx_bound = ctx_bound
         self.width = (ctx_bound + runner.page_size - 1) // runner.page_size
         n_groups = len(runner.cache.groups)
         # layout: tokens, positions, context_lens, state_slots | per group: table, slots
-        self.sizes = [rows, rows, rows, rows] + [rows * self.width] * n_groups + [rows] * n_groups + [rows] * adapters
+        self.sizes = [rows, rows, rows, rows] + [rows * self.width] * n_groups + [rows] * n_groups + \
+            [2 * self.RUNS + 1 + rows] * (shared is not None) + [rows] * adapters
         self.offs = np.cumsum([0] + self.sizes)
         total = int(self.offs[-1])
         # two pinned buffers taken in turn (the next step may be staged while the last copy is still queued),
@@ -124,7 +133,10 @@ class _DecodeGraph:
         ctx.block_tables = [self.view(4 + g).view(self.rows, self.width) for g in range(n_groups)]
         ctx.slot_mapping = [self.view(4 + n_groups + g) for g in range(n_groups)]
         if self.adapters:
-            ctx.adapter_ids = self.view(4 + 2 * n_groups)
+            ctx.adapter_ids = self.view(len(self.sizes) - 1)
+        if self.shared is not None:
+            ctx.shared_keys = ops.SharedKeys.captured(self.view(4 + 2 * n_groups), self.rows, self.RUNS, self.shared[0])
+            ctx.max_own_len = min(self.shared[1], self.width * runner.page_size)
         ctx.max_q_len = 1
         ctx.num_single = self.rows
         ctx.max_context_len = self.width * runner.page_size
@@ -193,6 +205,10 @@ class ModelRunner:
         self._adapter_staging = _PackedStaging(self.device)
         #: requests with an adapter -> its slot (whoever adds a request says so here, for as long as it runs)
         self.adapter_of: Dict[Hashable, int] = {}
+        # requests may begin with pages of another where nothing but the paged cache carries what came before
+        self.can_share = self.cache.shareable and not self.pools.state
+        self._key_bytes = max([g.page_bytes(1, 4 if (cache_dtype or model.dtype) == torch.float32 else 2) for g in model.cache_groups], default=0)
+        self._shared_keys: Dict[tuple, ops.SharedKeys] = {}
         #: host time spent packing the inputs of eager steps, and how many such steps there were
         self.host_seconds = {"pack": 0.0}
         self.host_steps = {"pack": 0}
@@ -322,15 +338,54 @@ class ModelRunner:
             ids = np.repeat(np.asarray([self.adapter_of.get(e.rid, -1) for e in entries], dtype=np.int32), n_new)
             self._adapter_staging.take(N)[:N] = ids
             ctx.adapter_ids = self._adapter_staging.send(N)
+        runs = self._shared_runs([e.rid for e in entries])
+        if runs is not None:
+            key = tuple(runs)
+            if key not in self._shared_keys:
+                if len(self._shared_keys) >= 64:
+                    self._shared_keys.clear()
+                self._shared_keys[key] = ops.SharedKeys([c for c, _ in runs], [v for _, v in runs], self.device)
+            ctx.shared_keys = self._shared_keys[key]
+            each = np.repeat([v for _, v in runs], [c for c, _ in runs])
+            ctx.max_own_len = int((ctx_lens - each).max())
         self.host_seconds["pack"] += time.perf_counter() - t_start
         self.host_steps["pack"] += 1
         return tok_dev, ctx
+
+    def _shared_runs(self, rids, most: Optional[int] = None):
+        """[(requests, shared keys)] of neighbours that begin with the same pages, or None where reading them once saves too little.
+        ``most``: so many runs at most that share keys, those that save most; the others' requests read theirs for themselves."""
+        if not self.cache._shared:
+            return None
+        runs, last = [], None
+        for rid in rids:
+            began = self.cache._shared.get(rid)
+            if began is not None and began == last:
+                runs[-1][0] += 1
+            else:
+                runs.append([1, 0 if began is None else began[1]])
+            last = began
+        runs = [(c, v if c > 1 else 0) for c, v in runs]
+        if most is not None and sum(1 for _, v in runs if v) > most:
+            best = set(sorted(range(len(runs)), key=lambda i: ((1 - runs[i][0]) * runs[i][1], i))[:most])
+            runs = [(c, v if i in best else 0) for i, (c, v) in enumerate(runs)]
+        saved = sum((c - 1) * v for c, v in runs)
+        return runs if saved * self._key_bytes >= ops.shared_keys_pay_bytes else None
 
     def _adapted(self, rids) -> bool:
         return bool(self.adapter_of) and any(rid in self.adapter_of for rid in rids)
 
     # ---- decode steps as a graph -----------------------------------------
-    def _graph_for(self, rows: int, ctx_len: int, adapters: bool = False) -> Optional[_DecodeGraph]:
+    def _shared_bounds(self, rids) -> Optional[tuple]:
+        """For a captured step: powers of two (from 256 on) that bound the shared keys and the keys behind them, or None."""
+        runs = self._shared_runs(rids, ops.SharedKeys.runs_in(_DecodeGraph.RUNS))
+        if runs is None:
+            return None
+        each = np.repeat([v for _, v in runs], [c for c, _ in runs])
+        own = max(self.cache.num_tokens(r) + 1 - int(v) for r, v in zip(rids, each))
+        return tuple(max(256, 1 << (n - 1).bit_length()) for n in (max(v for _, v in runs), own))
+
+    def _graph_for(self, rows: int, ctx_len: int, adapters: bool = False, shared: Optional[tuple] = None) -> Optional[_DecodeGraph]:
         # rows padded to a power of two, beyond 128 to a multiple of 128: the products see as many blocks of rows as
         # in the unpadded step and so choose the same tiles and parts of K (the same bits as an eager step)
         bucket = ops.decode_rows_padded(rows)
@@ -338,10 +393,13 @@ class ModelRunner:
         while bound < ctx_len:
             bound *= 2
         bound = min(bound, (self.model.spec.max_positions + self.page_size - 1) // self.page_size * self.page_size)
-        key = (bucket, bound, True) if adapters else (bucket, bound)
+        if shared is not None and shared[0] >= bound:      # (a bound on shared keys leaves room for a key behind them)
+            bound = min(2 * shared[0], (self.model.spec.max_positions + self.page_size - 1) // self.page_size * self.page_size)
+            shared = (min(shared[0], bound - 1), shared[1])
+        key = (bucket, bound) + ((True,) if adapters else ()) + (() if shared is None else (shared,))
         g = self._graphs.get(key)
         if g is None:
-            g = _DecodeGraph(self, bucket, bound, adapters)
+            g = _DecodeGraph(self, bucket, bound, adapters, shared)
             self._graphs[key] = g
         return g
 
@@ -351,6 +409,9 @@ class ModelRunner:
         g.copied[i].synchronize()                  # the last copy out of this pinned buffer has finished
         self.cache.fill_decode(rids, tokens, g.rows, g.width,
                                [self.pools.scratch_page(gi) for gi in range(len(self.cache.groups))], g.host_nps[i])
+        if g.shared is not None:
+            k = 4 + 2 * len(self.cache.groups)
+            ops.SharedKeys.pack(self._shared_runs(rids, ops.SharedKeys.runs_in(g.RUNS)), g.rows, g.RUNS, g.host_nps[i][int(g.offs[k]): int(g.offs[k + 1])])
         if g.adapters:
             ids = g.host_nps[i][int(g.offs[-2]):]
             ids[:] = -1
@@ -375,7 +436,7 @@ class ModelRunner:
             self.cache.reserve_many(rids, [1] * len(rids))
         except PagesExhausted:
             return False
-        g = self._graph_for(len(rids), ctx_len, self._adapted(rids))
+        g = self._graph_for(len(rids), ctx_len, self._adapted(rids), self._shared_bounds(rids))
         if g.graph is None:
             return False
         self._fill_graph_inputs(g, rids, [0] * len(rids))
@@ -400,7 +461,7 @@ class ModelRunner:
                 g.tok_copied.record()
         else:
             ctx_len = self.cache.max_num_tokens(rids) + 1
-            g = self._graph_for(n, ctx_len, self._adapted(rids))
+            g = self._graph_for(n, ctx_len, self._adapted(rids), self._shared_bounds(rids))
             self._fill_graph_inputs(g, rids, [0] * n if on_device else tokens)
         if on_device:
             g.packed[:n].copy_(tokens)

@@ -51,6 +51,9 @@ class Request:
     arrival: int = 0
     logprobs_top_n: Optional[int] = None     # not None: keep a log-probability record per generated token
     logprobs: List[object] = field(default_factory=list)
+    pages: int = 0                   # the most pages of a group that it holds for itself
+    #: (live request, tokens): this request begins with that one's first tokens and shares their pages while it has them
+    prefix: Optional[Tuple[Hashable, int]] = None
     _array: Optional[object] = field(default=None, repr=False, compare=False)
 
     @property
@@ -113,6 +116,8 @@ class Scheduler:
         self._arrivals = 0
         self.num_preemptions = 0
         self.pages_high_water = [0] * len(cache.pools)
+        #: pages of every group that are held for good beside the requests' own (prefixes that requests may begin with)
+        self.pages_kept = 0
 
     # ---- intake --------------------------------------------------------
     def add_request(self, req: Request) -> None:
@@ -140,9 +145,11 @@ class Scheduler:
             tokens_held = rule_of(spec.kind).held_tokens(spec, need_tokens, step)
             if tokens_held < need_tokens:
                 tokens_held = min(need_tokens, tokens_held + ps)
-            if (tokens_held + ps - 1) // ps > pool.num_pages:
+            need = (tokens_held + ps - 1) // ps - (req.prefix[1] // ps if req.prefix is not None else 0)
+            if need > pool.num_pages - self.pages_kept:
                 raise ValueError(
-                    f"request {req.rid!r}: needs {(tokens_held + ps - 1) // ps} pages of cache group {g}, the pool has {pool.num_pages}")
+                    f"request {req.rid!r}: needs {need} pages of cache group {g}, the pool has {pool.num_pages - self.pages_kept}")
+            req.pages = max(req.pages, need)
         req.arrival = self._arrivals
         self._arrivals += 1
         req.state = RequestState.WAITING
@@ -251,9 +258,13 @@ class Scheduler:
                 if len(self.cache.live_requests()) >= self.cache.max_requests:
                     break
                 self.cache.add(req.rid)
+                if req.prefix is not None and self.cache.has(req.prefix[0]):
+                    self.cache.share(req.rid, *req.prefix)
+                    req.num_computed = req.prefix[1]
             count = self._portion(req, budget)
             if count == 0 or not self._admissible(req, count, planned):
                 self.cache.release(req.rid)
+                req.num_computed = 0
                 break
             self.waiting.popleft()
             req.state = RequestState.RUNNING

@@ -1476,6 +1476,14 @@ def attention_rows(rows, col0: int, ctx, group: int, heads: int, kvh: int, dim: 
     return None if into is not None else out
 
 
+#: a step's shared keys are read once for all where that saves at least so many bytes of keys and values a layer.  (8 key heads of 128, single tokens, kernels
+#: alone, prefix / paged: 8 requests of 2,048 shared keys, 58 MB, 11.9 / 12.7 us, 2 and 4 of 4,096, 17 and 50 MB, 11.3 / 11.4 and 12.6 / 13.8, 8 of 8,192 19.0 / 27.4;
+#: besides, ``attention_rows`` takes the launch in front of the attention in, 3 us, and this one does not.)
+shared_keys_pay_bytes = 64 << 20
+#: steps whose rows' parts would take more bytes of scratch than this run ``paged_attention`` instead of ``prefix_attention``
+prefix_scratch_limit = 1 << 30
+
+
 class SharedKeys:
     """Which requests of a step begin with the same keys: the batch's requests in runs of ``counts[g]`` neighbours, the first
     ``lengths[g]`` keys of every request of run g lying in the same pages (0: they share nothing).  Requests behind the last
@@ -1499,9 +1507,47 @@ class SharedKeys:
         self.max_keys = max((v for _, v in runs), default=0)
         self.max_requests = max((c for c, v in runs if v), default=0)
         self.sharing = sum(1 for _, v in runs if v)
-        self._runs, self._plans = [(c, v) for c, v in runs if v], {}
+        self._runs, self._plans, self._bound = [(c, v) for c, v in runs if v], {}, False
         data = torch.tensor(starts + [v for _, v in runs] + [v for c, v in runs for _ in range(c)], dtype=torch.int32).to(device)
         self.starts, self.keys, self.each = data[: self.groups + 1], data[self.groups + 1: 2 * self.groups + 1], data[2 * self.groups + 1:]
+
+    @classmethod
+    def captured(cls, data: torch.Tensor, requests: int, groups: int, max_keys: int) -> "SharedKeys":
+        """For a captured step whose runs change from replay to replay: ``data`` (int32, device) holds what ``pack`` writes, ``groups`` runs of together
+        ``requests`` requests that share up to ``max_keys`` keys; launches are laid out for these bounds."""
+        self = cls.__new__(cls)
+        self.requests, self.groups, self.max_keys, self.max_requests = requests, groups, max_keys, requests
+        self.sharing = cls.runs_in(groups)
+        self._runs, self._plans, self._bound = [(requests, max_keys)], {}, True
+        _need(data.dtype == torch.int32 and data.numel() == 2 * groups + 1 + requests, "SharedKeys: data must be int32 [2 groups + 1 + requests]")
+        self.starts, self.keys, self.each = data[: groups + 1], data[groups + 1: 2 * groups + 1], data[2 * groups + 1:]
+        return self
+
+    @staticmethod
+    def runs_in(groups: int) -> int:
+        """How many runs that share keys ``captured`` has room for: one run of others in front of each, and one behind them all."""
+        return max(0, (groups - 1) // 2)
+
+    @staticmethod
+    def pack(runs, requests: int, groups: int, out) -> None:
+        """Runs [(requests, shared keys)], at most ``runs_in(groups)`` of them with shared keys, into ``out`` (int32 array
+        [2 groups + 1 + requests]) for ``captured``."""
+        merged = []
+        for c, v in list(runs) + [(requests - sum(c for c, _ in runs), 0)]:
+            _need(c >= 0 and v >= 0, "SharedKeys: more requests in runs than there are")
+            if merged and merged[-1][1] == 0 == v:
+                merged[-1][0] += c
+            elif c:
+                merged.append([c, v])
+        _need(len(merged) <= groups, "SharedKeys: more runs than there is room for")
+        out[:] = 0
+        at = 0
+        for i, (c, v) in enumerate(merged):
+            out[groups + 1 + i] = v
+            out[2 * groups + 1 + at: 2 * groups + 1 + at + c] = v
+            at += c
+            out[i + 1] = at
+        out[len(merged) + 1: groups + 1] = at
 
 
 def prefix_attention_ok(dtype: torch.dtype, heads: int, kvh: int, dim: int, value_dim: int, page_size: int, max_q_len: int) -> bool:
@@ -1575,7 +1621,10 @@ def _prefix_checked(q, k_cache, v_cache, block_tables, shared: SharedKeys, max_q
     rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts = _prefix_plan(shared, r, n, heads // kvh, kvh, max_q_len, own, d, q.dtype)
     sizes = (_dt(q), width, n, r, shared.groups, heads, kvh, d, page_size, max_q_len, rows_shared, rows_own, blocks, shared_steps, shared_parts,
              own_steps, own_parts)
-    return n, r, heads, (ctypes.c_int * len(sizes))(*sizes), n * heads * (shared_parts + own_parts) * (d + 2) + 2
+    room = n * heads * (shared_parts + own_parts) * (d + 2) + 2
+    if room * 4 > prefix_scratch_limit:
+        return n, r, heads, None, 0
+    return n, r, heads, (ctypes.c_int * len(sizes))(*sizes), room
 
 
 def _prefix_plan(shared: SharedKeys, r: int, n: int, group: int, kvh: int, max_q_len: int, own: int, dim: int, dtype: torch.dtype) -> tuple:
@@ -1587,7 +1636,7 @@ def _prefix_plan(shared: SharedKeys, r: int, n: int, group: int, kvh: int, max_q
     own_rows = 16 if max_q_len * group <= 16 else 64 if max_q_len * group <= 64 else 128
     rows = max(own_rows, 16 if most <= 16 else 64 if most <= 64 else 128)
     single = max_q_len == 1 and n == r
-    blocks = sum(-(-c * group // rows) for c, _ in shared._runs) if single else n * group // rows + shared.sharing
+    blocks = sum(-(-c * group // rows) for c, _ in shared._runs) if single and not shared._bound else n * group // rows + shared.sharing
     own_blocks = r * -(-max_q_len * group // own_rows)
     # Parts: as long as the launch would take if it were spread evenly, less what a block takes to begin and the join.  A step takes a
     # block that is alone on its CU step_us, two blocks twice that each; 5.5 TB/s is what single tokens' attention gets from memory.
@@ -1610,8 +1659,8 @@ def _prefix_plan(shared: SharedKeys, r: int, n: int, group: int, kvh: int, max_q
         parts = max(parts, min(-(-steps // 8), slots // (blocks * kvh)))
     parts = max(1, min(parts, 112, slots // (blocks * kvh)))
     per = -(-steps // parts)
-    # (own keys: two steps a wave, four where there are many blocks)
-    own_per = max(8 if own_blocks * kvh < 256 else 16, -(-own_steps // 16))
+    # (own keys: two steps a wave, four where there are many blocks; not in more parts than fill the chip a few times, which for portions is one)
+    own_per = max(8 if own_blocks * kvh < 256 else 16, -(-own_steps // max(1, min(16, 2048 // (own_blocks * kvh)))))
     return rows, own_rows, blocks, per, -(-steps // per), own_per, -(-own_steps // own_per)
 
 

@@ -302,9 +302,11 @@ class PagedAttention(TakesAdapters, Mixer):
         shared = getattr(ctx, "shared", None)      # (a context that a program made itself may share nothing)
         step = {**into, "shared": shared}
         a, attended = None, False
+        # (requests that begin with the same pages: keys that all of them see are read once)
+        shared_keys = getattr(ctx, "shared_keys", None) if self.window is None and not self.chunk and self.dist_table is None and not self.gate else None
         if q is None:
             rows = self._project(x, cache, rot) if ids is None else self._project_adapted(x, ids, ctx, cache)
-            if cache.writes and (rot is not None or type(self.position).__name__ == "NoPosition") and not self.softcap and self.dist_table is None \
+            if shared_keys is None and cache.writes and (rot is not None or type(self.position).__name__ == "NoPosition") and not self.softcap and self.dist_table is None \
                     and ops.attention_rows_ok(rows, ctx, self.num_heads, self.num_kv_heads, self.head_dim, self.value_dim, cache.k) \
                     and ops.attention_rows_pays(ctx, self.num_kv_heads, self.head_dim, int(self.window or 0), self.keep_first, self.chunk):
                 # single tokens: the attention takes the projection's rows itself
@@ -319,6 +321,10 @@ class PagedAttention(TakesAdapters, Mixer):
                 q = self._rotate(rows, ctx, cache, rot)
         if attended:
             pass
+        elif shared_keys is not None:
+            a = ops.prefix_attention(
+                q, cache.k, cache.v, ctx.block_tables[cache.group], ctx.cu_seqlens, ctx.context_lens, ctx.token_req, self.scale, shared_keys,
+                ctx.max_q_len, ctx.max_context_len, ctx.max_own_len, ctx.num_single, sink=self.sink_w, softcap=self.softcap)
         elif self.extended or self.chunk or self.softcap:
             a = ops.paged_attention(
                 q, cache.k, cache.v, ctx.block_tables[cache.group], ctx.cu_seqlens, ctx.context_lens,

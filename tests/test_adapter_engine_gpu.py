@@ -40,8 +40,8 @@ def test_greedy_generation_matches_plain(tiny_dirs, name, graph):
 
 @pytest.mark.parametrize("name", ["C", "D"])
 def test_bfloat16_logits_against_plain(tiny_dirs, name):
-    """Prompts and single tokens in bfloat16 against the plain model on merged weights, within the noise that the base model has (its products
-    round the same rows; the adapters' share is added to float32 sums)."""
+    """Prompts and single tokens in bfloat16 against the plain model on merged weights, within the bound that every bfloat16 engine test here is held to: a
+    small multiple of what rounding the stored rows of the same request to bfloat16 moves (the adapters' share is added to float32 sums and rounds no further row)."""
     from tempura_amd.engine import StepEntry
     cfg, W = tiny_dirs.plain_model(name, "bfloat16")
     pairs = adapter_cases.make(W, 4, rank=8, dtype=torch.bfloat16)
@@ -60,9 +60,9 @@ def test_bfloat16_logits_against_plain(tiny_dirs, name):
         got["x"].append((sx + cx - 1, logits[0]))
         got["y"].append((sy + cy - 1, logits[1]))
     for rid, t, weights in (("x", toks[0], adapter_cases.merged(W, pairs, 1.0)), ("y", toks[1], W)):
-        ref = plain.forward(cfg, weights, t)
-        for place, row in got[rid]:
-            assert helpers.rel_err(row, ref[place]) <= helpers.TOL["bfloat16"]
+        ref, bound = helpers.plain_reference(cfg, weights, t, "bfloat16")
+        places = [place for place, _ in got[rid]]
+        assert float((torch.stack([row for _, row in got[rid]]) - ref[places]).abs().max() / ref.abs().max()) <= bound
     for rid in got:
         r.end_request(rid)
 

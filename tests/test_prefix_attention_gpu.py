@@ -122,6 +122,44 @@ def test_the_same_call_gives_the_same_bits_on_any_stream_and_in_a_graph():
         t["ctx"].sub_((t["ctx"] > 600).to(torch.int32) * 7)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_runs_of_a_captured_step_move_between_replays(dtype):
+    """Launches laid out for bounds: other runs, lengths and tables with every replay, each against the definition."""
+    import numpy as np
+    from tempura_amd.kernels import ops
+    n, groups, bound, own_bound = 12, 17, 1024, 512
+    steps = [P.step(runs, [1 + (53 * i + 7 * k) % 500 for i in range(n)], [1] * n, 8, 2, 64, 16, dtype, seed=20 + k, spare=(1536 - bound) // 16)
+             for k, runs in enumerate([[(12, 1008)], [(1, 0), (5, 512), (6, 0)], [(2, 16 * j) for j in (1, 9, 30, 64, 2, 5)], [(12, 0)], [(3, 128), (9, 976)]])]
+    width, pages = 96, max(s["k"].shape[0] for s in steps)
+    t = {"q": steps[0]["q"].to(DEV), "k": torch.zeros((pages,) + steps[0]["k"].shape[1:], dtype=dtype, device=DEV), "ctx": torch.ones(n, dtype=torch.int32, device=DEV),
+         "v": torch.zeros((pages,) + steps[0]["v"].shape[1:], dtype=dtype, device=DEV), "tables": torch.zeros((n, width), dtype=torch.int32, device=DEV),
+         "starts": steps[0]["starts"].to(DEV), "req": steps[0]["req"].to(DEV)}
+    data = torch.zeros(2 * groups + 1 + n, dtype=torch.int32, device=DEV)
+    host = np.zeros(2 * groups + 1 + n, dtype=np.int32)
+    ops.SharedKeys.pack([], n, groups, host)
+    data.copy_(torch.from_numpy(host))
+    shared = ops.SharedKeys.captured(data, n, groups, bound)
+    call = lambda: ops.prefix_attention(t["q"], t["k"], t["v"], t["tables"], t["starts"], t["ctx"], t["req"], steps[0]["scale"], shared, 1, width * 16,  # noqa: E731
+                                        max_own_len=own_bound)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for s in steps + steps[::-1]:
+        for name in ("q", "k", "v", "ctx"):
+            t[name][: s[name].shape[0]].copy_(s[name])
+        t["tables"].fill_(-1)
+        wide = min(width, s["tables"].shape[1])
+        t["tables"][:, :wide].copy_(s["tables"][:, :wide])
+        ops.SharedKeys.pack(list(zip(s["counts"], s["lens"])), n, groups, host)
+        data.copy_(torch.from_numpy(host))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, size, reach = P.exact(s)
+        over = (out.cpu().double() - want).abs() - P.tolerance(s, want, size, reach)
+        assert bool(torch.isfinite(out).all()) and float(over.max()) <= 0, float(over.max())
+
+
 def test_tokens_that_are_not_there_are_not_written():
     """No tokens: nothing is launched.  A step's outputs are its own: the scratch of one call does not reach the next."""
     s = P.step([(3, 64)], [5, 6, 7], [1, 1, 1], 4, 2, 64, 16, BF16, seed=1)
