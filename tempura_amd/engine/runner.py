@@ -88,19 +88,20 @@ class _DecodeGraph:
     graphs are keyed by batch size with all per-step values device-read in the same way
     (/root/reference/engine/src/cutile_gpu_forward.rs:939-953)."""
 
-    #: runs of requests that a captured step has room for, eight of which may share keys
-    RUNS = 17
+    #: runs of requests that share keys in a captured step, at most (what a step has room for is a power of two up to this)
+    SHARING = 8
 
     def __init__(self, runner: "ModelRunner", rows: int, ctx_bound: int, adapters: bool = False, shared: Optional[tuple] = None):
         self.rows = rows
         self.adapters = adapters       # (the step's adapter slots lie behind everything else)
-        self.shared = shared           # (bounds on shared and own keys; the runs lie in front of the adapter slots)
+        self.shared = shared           # (bounds on shared and own keys and on the runs that share; the runs lie in front of the adapter slots)
+        self.runs = 0 if shared is None else 2 * shared[2] + 1      # (with the requests between and behind them)
         self.ctx_bound = ctx_bound
         self.width = (ctx_bound + runner.page_size - 1) // runner.page_size
         n_groups = len(runner.cache.groups)
         # layout: tokens, positions, context_lens, state_slots | per group: table, slots
         self.sizes = [rows, rows, rows, rows] + [rows * self.width] * n_groups + [rows] * n_groups + \
-            [2 * self.RUNS + 1 + rows] * (shared is not None) + [rows] * adapters
+            [2 * self.runs + 1 + rows] * (shared is not None) + [rows] * adapters
         self.offs = np.cumsum([0] + self.sizes)
         total = int(self.offs[-1])
         # two pinned buffers taken in turn (the next step may be staged while the last copy is still queued),
@@ -135,7 +136,7 @@ class _DecodeGraph:
         if self.adapters:
             ctx.adapter_ids = self.view(len(self.sizes) - 1)
         if self.shared is not None:
-            ctx.shared_keys = ops.SharedKeys.captured(self.view(4 + 2 * n_groups), self.rows, self.RUNS, self.shared[0])
+            ctx.shared_keys = ops.SharedKeys.captured(self.view(4 + 2 * n_groups), self.rows, self.runs, self.shared[0])
             ctx.max_own_len = min(self.shared[1], self.width * runner.page_size)
         ctx.max_q_len = 1
         ctx.num_single = self.rows
@@ -377,13 +378,14 @@ class ModelRunner:
 
     # ---- decode steps as a graph -----------------------------------------
     def _shared_bounds(self, rids) -> Optional[tuple]:
-        """For a captured step: powers of two (from 256 on) that bound the shared keys and the keys behind them, or None."""
-        runs = self._shared_runs(rids, ops.SharedKeys.runs_in(_DecodeGraph.RUNS))
+        """For a captured step: powers of two that bound the shared keys, the keys behind them (both from 256 on) and the runs that share, or None."""
+        runs = self._shared_runs(rids, _DecodeGraph.SHARING)
         if runs is None:
             return None
         each = np.repeat([v for _, v in runs], [c for c, _ in runs])
         own = max(self.cache.num_tokens(r) + 1 - int(v) for r, v in zip(rids, each))
-        return tuple(max(256, 1 << (n - 1).bit_length()) for n in (max(v for _, v in runs), own))
+        return tuple(max(256, 1 << (n - 1).bit_length()) for n in (max(v for _, v in runs), own)) \
+            + (1 << (sum(1 for _, v in runs if v) - 1).bit_length(),)
 
     def _graph_for(self, rows: int, ctx_len: int, adapters: bool = False, shared: Optional[tuple] = None) -> Optional[_DecodeGraph]:
         # rows padded to a power of two, beyond 128 to a multiple of 128: the products see as many blocks of rows as
@@ -395,7 +397,7 @@ class ModelRunner:
         bound = min(bound, (self.model.spec.max_positions + self.page_size - 1) // self.page_size * self.page_size)
         if shared is not None and shared[0] >= bound:      # (a bound on shared keys leaves room for a key behind them)
             bound = min(2 * shared[0], (self.model.spec.max_positions + self.page_size - 1) // self.page_size * self.page_size)
-            shared = (min(shared[0], bound - 1), shared[1])
+            shared = (min(shared[0], bound - 1),) + shared[1:]
         key = (bucket, bound) + ((True,) if adapters else ()) + (() if shared is None else (shared,))
         g = self._graphs.get(key)
         if g is None:
@@ -411,7 +413,7 @@ class ModelRunner:
                                [self.pools.scratch_page(gi) for gi in range(len(self.cache.groups))], g.host_nps[i])
         if g.shared is not None:
             k = 4 + 2 * len(self.cache.groups)
-            ops.SharedKeys.pack(self._shared_runs(rids, ops.SharedKeys.runs_in(g.RUNS)), g.rows, g.RUNS, g.host_nps[i][int(g.offs[k]): int(g.offs[k + 1])])
+            ops.SharedKeys.pack(self._shared_runs(rids, g.SHARING), g.rows, g.runs, g.host_nps[i][int(g.offs[k]): int(g.offs[k + 1])])
         if g.adapters:
             ids = g.host_nps[i][int(g.offs[-2]):]
             ids[:] = -1

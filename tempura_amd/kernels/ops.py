@@ -1476,10 +1476,11 @@ def attention_rows(rows, col0: int, ctx, group: int, heads: int, kvh: int, dim: 
     return None if into is not None else out
 
 
-#: a step's shared keys are read once for all where that saves at least so many bytes of keys and values a layer.  (8 key heads of 128, single tokens, kernels
-#: alone, prefix / paged: 8 requests of 2,048 shared keys, 58 MB, 11.9 / 12.7 us, 2 and 4 of 4,096, 17 and 50 MB, 11.3 / 11.4 and 12.6 / 13.8, 8 of 8,192 19.0 / 27.4;
-#: besides, ``attention_rows`` takes the launch in front of the attention in, 3 us, and this one does not.)
-shared_keys_pay_bytes = 64 << 20
+#: a step's shared keys are read once for all where that saves at least so many bytes of keys and values a layer.  (Single tokens behind shared keys, 32 heads
+#: of 128 over 8 key heads, bf16, a layer of a captured step, once for all / each for itself, the projections and ``attention_rows``' own work among it:
+#: 2 requests of 8,192 keys, 34 MB, 138 / 135 us; 4 of 4,096, 50 MB, 135 / 135; 8 of 2,048, 59 MB, 137 / 138; 32 of 1,024, 130 MB, 174 / 169;
+#: 32 of 2,048, 260 MB, 174 / 175; 64 of 1,024, 264 MB, 182 / 186; 8 of 8,192, 235 MB, 143 / 153; 32 of 8,192, 1,040 MB, 183 / 215.)
+shared_keys_pay_bytes = 192 << 20
 #: steps whose rows' parts would take more bytes of scratch than this run ``paged_attention`` instead of ``prefix_attention``
 prefix_scratch_limit = 1 << 30
 
@@ -1636,7 +1637,8 @@ def _prefix_plan(shared: SharedKeys, r: int, n: int, group: int, kvh: int, max_q
     own_rows = 16 if max_q_len * group <= 16 else 64 if max_q_len * group <= 64 else 128
     rows = max(own_rows, 16 if most <= 16 else 64 if most <= 64 else 128)
     single = max_q_len == 1 and n == r
-    blocks = sum(-(-c * group // rows) for c, _ in shared._runs) if single and not shared._bound else n * group // rows + shared.sharing
+    blocks = sum(-(-c * group // rows) for c, _ in shared._runs) if single and not shared._bound else \
+        (n * group - shared.sharing) // rows + shared.sharing
     own_blocks = r * -(-max_q_len * group // own_rows)
     # Parts: as long as the launch would take if it were spread evenly, less what a block takes to begin and the join.  A step takes a
     # block that is alone on its CU step_us, two blocks twice that each; 5.5 TB/s is what single tokens' attention gets from memory.

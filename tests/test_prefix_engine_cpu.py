@@ -249,5 +249,5 @@ def test_a_captured_step_keeps_the_runs_that_save_most(tiny_dirs, emu):
     assert runner._shared_runs(rids) == [(2, 16 * (g + 1)) for g in range(10)]
     kept = runner._shared_runs(rids, 8)
     assert kept == [(2, 16 * (g + 1) if g >= 2 else 0) for g in range(10)]
-    shared, own = runner._shared_bounds(rids)
-    assert shared == 256 and own == 256      # (keys for themselves: 17 to 33)
+    assert runner._shared_bounds(rids) == (256, 256, 8)      # (keys for themselves: 17 to 33)
+    assert runner._shared_bounds(rids[:6]) == (256, 256, 4) and runner._shared_bounds(rids[:2]) == (256, 256, 1)
