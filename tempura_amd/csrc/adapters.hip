@@ -6,6 +6,8 @@
 //
 // Ranks are padded to a multiple of 8 with zeros.  The low-rank row v = A x stays float32: the result is a float32 sum of products of the
 // operands as they are, like the shared product's.
+#include <type_traits>
+
 #include "common.h"
 
 #define AD_MAX_SLICES 8
@@ -30,28 +32,57 @@ __device__ inline int slice_of(const AdapterArgs& a, int n) {
   return s;
 }
 
-// eight neighbouring elements as floats (VEC: at an address aligned to eight elements)
+// eight neighbouring elements as floats (VEC: at an address aligned to 16 bytes; else at any that an element may have, which global loads here allow)
 template <typename T, bool VEC>
-__device__ inline void load8(const T* p, int left, float (&v)[8]) {
+__device__ inline void load8(const T* p, float (&v)[8]) {
   if constexpr (VEC) {
     const float4 lo = load_float4(p), hi = load_float4(p + 4);
     v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
     v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
   } else {
+    T e[8];
+    __builtin_memcpy(e, p, sizeof(e));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_float(p[i]) : 0.f;
+    for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
   }
 }
 
 // ---- a few rows ------------------------------------------------------------------------------
+// sum[i] = A[i, :] . x over a wave's lanes, eight elements a lane at a time (lane 64 / R * i of the result holds the i-th)
+template <typename T, bool VEC, int R>
+__device__ inline float wave_dots(const T* A, const T* x, int K) {
+  const int lane = threadIdx.x & 63;
+  float sum[R] = {};
+  int k = lane * 8;
+#pragma unroll 8 / R
+  for (; k + 8 <= K; k += 512) {
+    float xv[8];
+    load8<T, VEC>(x + k, xv);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float av[8];
+      load8<T, VEC>(A + (size_t)i * K + k, av);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum[i] = fmaf(av[e], xv[e], sum[i]);
+    }
+  }
+  if constexpr (!VEC) {      // (the elements behind the last eight, in the lane whose turn they are)
+    for (int n = k; n < K && n < k + 8; ++n) {
+#pragma unroll
+      for (int i = 0; i < R; ++i) sum[i] = fmaf(to_float(A[(size_t)i * K + n]), to_float(x[n]), sum[i]);
+    }
+  }
+  return wave_sums<R>(sum);
+}
+
 // A block takes one row and `cols` columns and works the row's low-rank values out for itself, those of its columns' slices: one launch
 // instead of two, which costs each block rank * K elements of A from the L2 (128 KB with rank 16 and K = 4,096, 2 us of a CU's path), asked for by
-// sixteen waves at once.
+// sixteen waves at once.  DONE: `low` [rows, slices * rank] holds them already (adapter_rows_down_kernel).
 // grid: (ceil(N / cols), rows).  v: LDS.
 #define AD_ROW_THREADS 1024
 // R: ranks of a wave at a time.
-template <typename T, bool VEC, int R>
-__global__ __launch_bounds__(AD_ROW_THREADS) void adapter_rows_kernel(AdapterArgs a, int cols) {
+template <typename T, bool VEC, int R, bool DONE>
+__global__ __launch_bounds__(AD_ROW_THREADS) void adapter_rows_kernel(AdapterArgs a, const float* __restrict__ low, int cols) {
   extern __shared__ float v[];          // [slices of these columns, rank]
   const int row = blockIdx.y, n0 = blockIdx.x * cols, n1 = min(n0 + cols, a.N);
   const int slot = a.ids[row];
@@ -59,50 +90,47 @@ __global__ __launch_bounds__(AD_ROW_THREADS) void adapter_rows_kernel(AdapterArg
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int s0 = a.interleaved ? 0 : slice_of(a, n0), s1 = a.interleaved ? 1 : slice_of(a, n1 - 1);
   const int ranks = (s1 - s0 + 1) * a.rank;
-  const T* x = (const T*)a.x + (size_t)row * a.K;
-  const T* A = (const T*)a.a + ((size_t)slot * a.slices + s0) * a.rank * a.K;
   // (a thread's column: its sum so far and its weights travel beside A)
   const int n = n0 + (int)threadIdx.x;
   const T* B = (const T*)a.b + ((size_t)slot * a.N + min(n, n1 - 1)) * a.rank;
   float first[8];
-  load8<T, true>(B, 8, first);
+  load8<T, true>(B, first);
   const float scale = a.scale[slot];
   float* y = a.y + (size_t)row * a.N;
   const float old = n < n1 ? y[n] : 0.f;
-  for (int j = wave * R; j < ranks; j += R * (AD_ROW_THREADS / 64)) {
-    float sum[R] = {};
-#pragma unroll(VEC ? 8 / R : 1)
-    for (int k = lane * 8; k < a.K; k += 512) {
-      float xv[8];
-      load8<T, VEC>(x + k, a.K - k, xv);
-#pragma unroll
-      for (int i = 0; i < R; ++i) {
-        float av[8];
-        load8<T, VEC>(A + (size_t)(j + i) * a.K + k, a.K - k, av);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum[i] = fmaf(av[e], xv[e], sum[i]);
-      }
+  if constexpr (DONE) {
+    for (int j = threadIdx.x; j < ranks; j += blockDim.x) v[j] = low[((size_t)row * a.slices + s0) * a.rank + j];
+  } else {
+    const T* x = (const T*)a.x + (size_t)row * a.K;
+    const T* A = (const T*)a.a + ((size_t)slot * a.slices + s0) * a.rank * a.K;
+    for (int j = wave * R; j < ranks; j += R * (AD_ROW_THREADS / 64)) {
+      const float total = wave_dots<T, VEC, R>(A + (size_t)j * a.K, x, a.K);
+      if (lane % (64 / R) == 0) v[j + lane / (64 / R)] = total;
     }
-    const float total = wave_sums<R>(sum);      // (lane 64 / R * i: the i-th)
-    if (lane % (64 / R) == 0) v[j + lane / (64 / R)] = total;
   }
   __syncthreads();
-  for (int c = n; c < n1; c += AD_ROW_THREADS) {
-    const float* vs = v + (slice_of(a, c) - s0) * a.rank;
-    float sum = 0.f;
-    for (int j = 0; j < a.rank; j += 8) {
-      float bv[8];
-      if (c == n && j == 0) {
+  if (n >= n1) return;
+  const float* vs = v + (slice_of(a, n) - s0) * a.rank;
+  float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) bv[e] = first[e];
-      } else {
-        load8<T, true>((const T*)a.b + ((size_t)slot * a.N + c) * a.rank + j, 8, bv);
-      }
+  for (int e = 0; e < 8; ++e) sum = fmaf(first[e], vs[e], sum);
+  for (int j = 8; j < a.rank; j += 8) {
+    float bv[8];
+    load8<T, true>(B + j, bv);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sum = fmaf(bv[e], vs[j + e], sum);
-    }
-    y[c] = fmaf(scale, sum, c == n ? old : y[c]);
+    for (int e = 0; e < 8; ++e) sum = fmaf(bv[e], vs[j + e], sum);
   }
+  y[n] = fmaf(scale, sum, old);
+}
+
+// low[row, ranks] = A x of rows taken one by one, a rank a wave: where A's rows are so long, or so many, that a block of the kernel above would be busy
+// with them for long.  grid: (ceil(ranks / 4), rows)
+template <typename T, bool VEC>
+__global__ __launch_bounds__(256) void adapter_rows_down_kernel(AdapterArgs a, float* __restrict__ low) {
+  const int row = blockIdx.y, slot = a.ids[row], ranks = a.slices * a.rank, j = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (slot < 0 || slot >= a.slots || j >= ranks) return;
+  const float total = wave_dots<T, VEC, 1>((const T*)a.a + ((size_t)slot * ranks + j) * a.K, (const T*)a.x + (size_t)row * a.K, a.K);
+  if ((threadIdx.x & 63) == 0) low[(size_t)row * ranks + j] = total;
 }
 
 // ---- many rows -------------------------------------------------------------------------------
@@ -137,21 +165,25 @@ __device__ inline int window_rows(const AdapterArgs& a, int window, int which, i
   return (int)__popcll(same);
 }
 
-// 16 bytes of a row from element k on, zeros behind its end (VEC: aligned, and the end is a multiple of the piece)
-template <typename T, bool VEC>
+// 16 bytes of a row from element k on, zeros behind its end (VEC: aligned, and the end is a multiple of the piece; FULL: the end is not in reach)
+template <typename T, bool VEC, bool FULL>
 __device__ inline ad_u32x4 load_piece(const T* row, int k, int K) {
   constexpr int P = 16 / sizeof(T);
   if constexpr (VEC) {
-    return k < K ? *(const ad_u32x4*)(row + k) : (ad_u32x4){0, 0, 0, 0};
+    return FULL || k < K ? *(const ad_u32x4*)(row + k) : (ad_u32x4){0, 0, 0, 0};
   } else {
     union {
       T e[P];
       ad_u32x4 v;
     } u;
+    if constexpr (FULL) {
+      __builtin_memcpy(u.e, row + k, 16);
+    } else {
 #pragma unroll
-    for (int i = 0; i < P; ++i) {
-      u.e[i] = T{};
-      if (k + i < K) u.e[i] = row[k + i];
+      for (int i = 0; i < P; ++i) {
+        u.e[i] = T{};
+        if (k + i < K) u.e[i] = row[k + i];
+      }
     }
     return u.v;
   }
@@ -199,21 +231,24 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(AdapterArgs a, float*
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int t = 0; t < 4; ++t) acc[i][t] = (ad_f32x4){0.f, 0.f, 0.f, 0.f};
-    for (int k = k0 + wave * STEP; k < k1; k += 4 * STEP) {
+    auto step = [&](int k, auto full) __attribute__((always_inline)) {
       const int at = k + g * (STEP / 4);
       ad_u32x4 xf[4], af[RT];
 #pragma unroll
-      for (int i = 0; i < RT; ++i) af[i] = load_piece<T, VEC>(ar[i], at, k1);
+      for (int i = 0; i < RT; ++i) af[i] = load_piece<T, VEC, full.value>(ar[i], at, k1);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
-        if (t < tiles) xf[t] = load_piece<T, VEC>(xr[t], at, k1);
+        if (t < tiles) xf[t] = load_piece<T, VEC, full.value>(xr[t], at, k1);
 #pragma unroll
       for (int t = 0; t < 4; ++t)
         if (t < tiles) {
 #pragma unroll
           for (int i = 0; i < RT; ++i) mfma_piece<T>(af[i], xf[t], acc[i][t]);
         }
-    }
+    };
+    int k = k0 + wave * STEP;
+    for (; k + STEP <= k1; k += 4 * STEP) step(k, std::true_type{});
+    if (k < k1) step(k, std::false_type{});
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       if (t >= tiles) break;
@@ -493,8 +528,9 @@ static void adapter_many(const AdapterArgs& g, int parts, int vec, int write, fl
 }
 
 // y [rows, N] float32 += the adapters' share.  a [slots, slices * rank, K], b [slots, N, rank] of dt, rank a multiple of 8; vec: K is a multiple of
-// 8 and x and a are aligned to 16 bytes.  ends: the columns at which the slices end (the last is N).  parts 0: a block a row; else rows taken
-// together by adapter, K in up to `parts` parts, with scratch of parts * rows * slices * rank floats aligned to 16 bytes; `write`: y is written
+// 8 and x and a are aligned to 16 bytes.  ends: the columns at which the slices end (the last is N).  parts 0: row by row, in one launch, or with
+// scratch of rows * slices * rank floats in two; else rows taken together by adapter, K in up to `parts` parts, with scratch of parts times as many floats
+// aligned to 16 bytes; `write`: y is written
 // instead (zeros for rows without an adapter).
 extern "C" int tp_adapter_add(const int* ids, const void* x, int dt, const void* a, const void* b, const float* scale, float* y, int rows, int K, int N,
                               int slots, int rank, int slices, int interleaved, const int* ends, int vec, int parts, int write, float* scratch, hipStream_t s) {
@@ -519,14 +555,23 @@ extern "C" int tp_adapter_add(const int* ids, const void* x, int dt, const void*
   const dim3 grid((N + cols - 1) / cols, rows);
   const size_t lds = (size_t)slices * rank * sizeof(float);
   TP_REQUIRE(lds <= 65536, "adapter_add: ranks of all slices beyond 16,384");
-#define AD_ROWS(T, VEC) (rank <= 16 ? adapter_rows_kernel<T, VEC, 1><<<grid, AD_ROW_THREADS, lds, s>>>(g, cols) \
-                                    : adapter_rows_kernel<T, VEC, 2><<<grid, AD_ROW_THREADS, lds, s>>>(g, cols))
-  if (dt == TP_BF16) {
-    if (vec) AD_ROWS(bf16_t, true);
-    else AD_ROWS(bf16_t, false);
+#define AD_ROWS(T, VEC)                                                                                                     \
+  if (scratch != nullptr) {                                                                                                 \
+    adapter_rows_down_kernel<T, VEC><<<dim3((slices * rank + 3) / 4, rows), 256, 0, s>>>(g, scratch);                       \
+    adapter_rows_kernel<T, VEC, 1, true><<<grid, cols, lds, s>>>(g, scratch, cols);                                         \
+  } else if (rank <= 16) {                                                                                                  \
+    adapter_rows_kernel<T, VEC, 1, false><<<grid, AD_ROW_THREADS, lds, s>>>(g, nullptr, cols);                              \
+  } else {                                                                                                                  \
+    adapter_rows_kernel<T, VEC, 2, false><<<grid, AD_ROW_THREADS, lds, s>>>(g, nullptr, cols);                              \
+  }
+  if (dt == TP_BF16 && vec) {
+    AD_ROWS(bf16_t, true)
+  } else if (dt == TP_BF16) {
+    AD_ROWS(bf16_t, false)
+  } else if (vec) {
+    AD_ROWS(float, true)
   } else {
-    if (vec) AD_ROWS(float, true);
-    else AD_ROWS(float, false);
+    AD_ROWS(float, false)
   }
 #undef AD_ROWS
   TP_CHECK_LAUNCH("adapter_add");

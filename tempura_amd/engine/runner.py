@@ -339,7 +339,7 @@ class ModelRunner:
             ids = np.repeat(np.asarray([self.adapter_of.get(e.rid, -1) for e in entries], dtype=np.int32), n_new)
             self._adapter_staging.take(N)[:N] = ids
             ctx.adapter_ids = self._adapter_staging.send(N)
-        runs = self._shared_runs([e.rid for e in entries])
+        runs = self._shared_runs([e.rid for e in entries], longest=max_q)
         if runs is not None:
             key = tuple(runs)
             if key not in self._shared_keys:
@@ -353,9 +353,10 @@ class ModelRunner:
         self.host_steps["pack"] += 1
         return tok_dev, ctx
 
-    def _shared_runs(self, rids, most: Optional[int] = None):
+    def _shared_runs(self, rids, most: Optional[int] = None, longest: int = 1):
         """[(requests, shared keys)] of neighbours that begin with the same pages, or None where reading them once saves too little.
-        ``most``: so many runs at most that share keys, those that save most; the others' requests read theirs for themselves."""
+        ``most``: so many runs at most that share keys, those that save most; the others' requests read theirs for themselves.
+        ``longest``: the tokens of the longest portion."""
         if not self.cache._shared:
             return None
         runs, last = [], None
@@ -371,7 +372,7 @@ class ModelRunner:
             best = set(sorted(range(len(runs)), key=lambda i: ((1 - runs[i][0]) * runs[i][1], i))[:most])
             runs = [(c, v if i in best else 0) for i, (c, v) in enumerate(runs)]
         saved = sum((c - 1) * v for c, v in runs)
-        return runs if saved * self._key_bytes >= ops.shared_keys_pay_bytes else None
+        return runs if saved > 0 and ops.shared_keys_pay(saved * self._key_bytes, longest) else None
 
     def _adapted(self, rids) -> bool:
         return bool(self.adapter_of) and any(rid in self.adapter_of for rid in rids)

@@ -894,8 +894,18 @@ def linear(x, w: torch.Tensor, out_dtype: torch.dtype, residual: Optional[torch.
 ADAPTER_SLICES = 8
 
 
-#: steps of up to this many rows have a block a row and 256 columns work out its low-rank values for itself (of single tokens four times as many)
-adapter_single_rows = 32
+#: rows are taken one by one up to this many, single tokens up to that many,
+adapter_row_limits = (256, 512)
+#: where no more than so many bytes of adapters' weights are read that way, and so many more for each adapter that single tokens may have; else
+#: rows with the same adapter are taken together.  (us beside the shared product, rank x K, 4,096 columns, bf16, one by one / together: 128 rows of
+#: 4 adapters, 32 x 4,096 10.5 / 11.9, 64 x 4,096 19.4 / 12.9, 16 x 14,336 12.0 / 14.4, 32 x 14,336 19.9 / 15.0; 192 rows, 32 x 1,024 11.7 / 10.8, 16 x 4,096
+#: 10.1 / 12.1.  Of
+#: 32 adapters, which then share a window of 64 rows: 128 rows of 64 x 4,096 31 / 39, 256 57 / 58, 512 99 / 93.)
+adapter_row_weights, adapter_row_weights_each = 64 << 20, 8 << 20
+#: rows one by one: a launch works their low-rank values out in front where one block would read more than this of A for its row, or all blocks
+#: more than that.  (One launch / two, 16 rows, rank x K: 16 x 4,096 6.0 / 6.7 us, 16 x 8,192 8.0 / 8.1, 64 x 4,096 11.7 / 8.6, 16 x 14,336 11 / 10;
+#: 8 x 4,096 in 768 blocks, 50 MB, 9.1 / 9.5, in 2,048, 134 MB, 18.1 / 16.1, 16 x 4,096 in 512, 67 MB, 9.0 / 8.5.)
+adapter_block_bytes, adapter_blocks_bytes = 192 << 10, 48 << 20
 
 
 class Adapters:
@@ -951,26 +961,28 @@ def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, re
         raise KernelError(f"adapter_linear: shapes {(m, k)} x {tuple(w.shape)} with adapters of {adapters.k} x {adapters.n}")
     _need(ids.dtype == torch.int32 and ids.dim() == 1 and ids.numel() == m, "adapter_linear: ids must be int32 [m]")
     _need(x.device == ids.device == adapters.a.device, "adapter_linear: operands on different devices")
-    if m == 0 or not (m > adapter_single_rows if max_run != 1 else m > 4 * adapter_single_rows):
+    if m == 0:
+        return linear(x, w, torch.float32, residual=residual)
+    # (single tokens by the rows that a captured step of as many has, for the same bits)
+    rows, ranks, size = decode_rows_padded(m) if max_run == 1 else m, adapters.slices * adapters.rank, x.element_size()
+    most = adapter_row_weights + (adapter_row_weights_each * min(adapters.slots, 64) if max_run == 1 else 0)
+    if rows <= adapter_row_limits[max_run == 1] and rows * (ranks * k + adapters.rank * adapters.n) * size <= most:
+        two = adapters.rank * k * size > adapter_block_bytes or rows * -(-adapters.n // 1024) * adapters.rank * k * size > adapter_blocks_bytes
         y = linear(x, w, torch.float32, residual=residual)
-        if m:
-            _adapter_add(x, adapters, ids, y, 0, 0)
+        _adapter_add(x, adapters, ids, y, 0, 0, two)
         return y
     # (many rows: the adapters' share first, onto which the shared product adds its own: it reads y in its epilogue, 118.4 -> 124.0 us for 4,096
     # rows of 4,096 x 4,096 and nothing for 731 of 8,192 x 2,048, where the other order reads it in a pass of its own, 17 us)
     y = torch.empty((m, adapters.n), dtype=torch.float32, device=x.device) if residual is None else residual
-    ranks = adapters.slices * adapters.rank
-    # (single tokens by the rows that a captured step of as many has: the order of a row's sums hangs on the parts of K)
-    windows = -(-(decode_rows_padded(m) if max_run == 1 else m) // 64)
-    parts = max(1, min(8, k // 512, 256 // (windows * -(-ranks // 64))))
+    parts = max(1, min(8, k // 512, 256 // (-(-rows // 64) * -(-ranks // 64))))
     _adapter_add(x, adapters, ids, y, parts, int(residual is None))
     return linear(x, w, torch.float32, residual=y)
 
 
-def _adapter_add(x: torch.Tensor, adapters: Adapters, ids: torch.Tensor, y: torch.Tensor, parts: int, write: int) -> None:
+def _adapter_add(x: torch.Tensor, adapters: Adapters, ids: torch.Tensor, y: torch.Tensor, parts: int, write: int, two: bool = False) -> None:
     m, k = x.shape
     _need(y.dtype == torch.float32 and tuple(y.shape) == (m, adapters.n), "adapter_linear: residual must be float32 [m, n]")
-    scratch = torch.empty((parts * m * adapters.slices * adapters.rank,), dtype=torch.float32, device=x.device) if parts else None
+    scratch = torch.empty((max(parts, 1) * m * adapters.slices * adapters.rank,), dtype=torch.float32, device=x.device) if parts or two else None
     vec = int(k % 8 == 0 and x.data_ptr() % 16 == 0 and adapters.a.data_ptr() % 16 == 0)
     _call("tp_adapter_add", _ptr(ids), _ptr(x), _dt(x), _ptr(adapters.a), _ptr(adapters.b), _ptr(adapters.scales), _ptr(y), m, k, adapters.n,
           adapters.slots, adapters.rank, adapters.slices, int(adapters.interleaved), adapters.ends, vec, parts, write, _ptr(scratch), _stream(),
@@ -1476,11 +1488,31 @@ def attention_rows(rows, col0: int, ctx, group: int, heads: int, kvh: int, dim: 
     return None if into is not None else out
 
 
-#: a step's shared keys are read once for all where that saves at least so many bytes of keys and values a layer.  (Single tokens behind shared keys, 32 heads
-#: of 128 over 8 key heads, bf16, a layer of a captured step, once for all / each for itself, the projections and ``attention_rows``' own work among it:
+#: the engine's steps of single tokens, and of portions of up to 128, read shared keys once for all where that saves at least so many bytes of keys and
+#: values a layer; of longer portions as many times more as they are longer, of portions up to 64 a twelfth.  (Single tokens behind shared keys, 32 heads of
+#: 128 over 8 key heads, bf16, a layer of a captured step, once for all / each for itself, the projections and ``attention_rows``' own work among it:
 #: 2 requests of 8,192 keys, 34 MB, 138 / 135 us; 4 of 4,096, 50 MB, 135 / 135; 8 of 2,048, 59 MB, 137 / 138; 32 of 1,024, 130 MB, 174 / 169;
-#: 32 of 2,048, 260 MB, 174 / 175; 64 of 1,024, 264 MB, 182 / 186; 8 of 8,192, 235 MB, 143 / 153; 32 of 8,192, 1,040 MB, 183 / 215.)
+#: 32 of 2,048, 260 MB, 174 / 175; 64 of 1,024, 264 MB, 182 / 186; 8 of 8,192, 235 MB, 143 / 153; 32 of 8,192, 1,040 MB, 183 / 215.  The attention alone of
+#: 4 and 32 tokens behind 2,048 or 8,192 keys beside a prompt of its own: 4 x 2,048 and 64 tokens, 25 MB, 17.7 / 23.0; 4 x 8,192 and 512, 100 MB, 80 / 56;
+#: 32 x 8,192 and 512, 91 / 112, and 2,048, 258 / 152.)
 shared_keys_pay_bytes = 192 << 20
+
+
+def shared_keys_pay(saved_bytes: int, longest: int) -> bool:
+    """Whether a step whose longest portion has ``longest`` tokens reads shared keys once for all, which saves so many bytes a layer."""
+    least = shared_keys_pay_bytes
+    return saved_bytes >= (least if longest == 1 else least // 12 if longest <= 64 else least * max(128, longest) // 128)
+
+
+#: shared keys are read once for all where a run shares at least so many (of single tokens, bf16 and float32; of others at least the third and sixteen for
+#: each token of the longest portion), or where single tokens are saved so many keys in all; for fewer the second launch, which joins the parts, or the
+#: many rows that own keys are read for, cost more than that saves.  (32 heads of 128 over 8, once for all / each for itself, single tokens, 100 keys
+#: of their own: 4 requests of 512, 1,024 and 2,048 keys 10.9 / 8.4, 11.0 / 9.5 and 11.5 / 10.8 us (and 14 / 19 for the host that calls), 16 of them
+#: 11.2 / 8.4, 12.7 / 13.3 and 14.0 / 18.2, 64 of 512 and 768 15.0 / 14.3 and
+#: 16.4 / 17.3; float32, 8 of 256, 768, 2,048 18.0 / 13.0, 18.4 / 17.1, 19.8 / 27.3.  Portions: 8 of 4 tokens behind 64, 256, 1,024 keys
+#: 10.6 / 9.6, 12.1 / 13.9, 14.2 / 33.6; of 64 behind 256, 1,024, 4,096 27 / 16, 42 / 35, 69 / 75; of 256 behind 1,024 and 4,096 104 / 88, 216 / 261;
+#: of 512 behind 4,096 450 / 408, 4 of 512 behind 8,192 342 / 438.)
+prefix_least_keys, prefix_least_saved = (768, 512, 192), 48 << 10
 #: steps whose rows' parts would take more bytes of scratch than this run ``paged_attention`` instead of ``prefix_attention``
 prefix_scratch_limit = 1 << 30
 
@@ -1565,7 +1597,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     that the requests of a run of ``shared`` have in common are read once for all of them.  Every request's block table names its shared pages
     as well; its new tokens lie behind its shared keys.  ``max_own_len``: the most keys that a request has behind its shared ones, its
     new tokens among them (a bound, at least the longest; None: ``max_context_len``).  Sizes that the kernel is not built for
-    (``prefix_attention_ok``), and steps without shared keys, run ``paged_attention``."""
+    (``prefix_attention_ok``), and steps without shared keys or with few (``prefix_least_keys``), run ``paged_attention``."""
     if _backend is not None:
         return _backend.prefix_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, shared, max_q_len,
                                          max_context_len, max_own_len, num_single, sink, softcap)
@@ -1618,6 +1650,10 @@ def _prefix_checked(q, k_cache, v_cache, block_tables, shared: SharedKeys, max_q
     _need(max_context_len <= width * page_size, "prefix_attention: block table narrower than the longest context")
     _need(shared.max_keys < max(1, max_context_len), "prefix_attention: a request's new tokens must lie behind its shared keys")
     if shared.max_keys == 0 or not prefix_attention_ok(q.dtype, heads, kvh, d, vd, page_size, max_q_len):
+        return n, r, heads, None, 0
+    least = prefix_least_keys[int(q.dtype == torch.float32)] if max_q_len == 1 else max(prefix_least_keys[2], min(prefix_least_keys[2], 16) * max_q_len)
+    many = max_q_len == 1 and sum((c - 1) * v for c, v in shared._runs) >= prefix_least_saved
+    if shared.max_keys < least and not many and not shared._bound:
         return n, r, heads, None, 0
     rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts = _prefix_plan(shared, r, n, heads // kvh, kvh, max_q_len, own, d, q.dtype)
     sizes = (_dt(q), width, n, r, shared.groups, heads, kvh, d, page_size, max_q_len, rows_shared, rows_own, blocks, shared_steps, shared_parts,

@@ -172,8 +172,9 @@ def test_adapter_refusals(calls):
     assert wide.rank == 8 and tuple(wide.a.shape) == (2, 16, 64) and tuple(wide.b.shape) == (2, 48, 8)
 
 
-def test_shared_keys_refusals(calls):
+def test_shared_keys_refusals(calls, monkeypatch):
     from tempura_amd.kernels import ops
+    monkeypatch.setattr(ops, "prefix_least_keys", (0, 0, 0))
     from tempura_amd.kernels.ops import KernelError
     i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
     good = dict(q=torch.zeros(3, 4, 64), k=torch.zeros(9, 2, 16, 64), v=torch.zeros(9, 2, 64, 16), t=torch.zeros(3, 6, dtype=torch.int32), cu=i32(0, 1, 2, 3),

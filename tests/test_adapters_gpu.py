@@ -58,6 +58,18 @@ def _check(case, residual=None, **more):
     return got
 
 
+@pytest.fixture(params=["rule", "one launch", "two launches", "together"])
+def way(request, monkeypatch):
+    """Rows one by one in a launch or in two, and together by adapter, whatever the rule on sizes would take."""
+    from tempura_amd.kernels import ops
+    if request.param != "rule":
+        monkeypatch.setattr(ops, "adapter_row_limits", (0, 0) if request.param == "together" else (1 << 16, 1 << 16))
+        monkeypatch.setattr(ops, "adapter_row_weights", 1 << 40)
+        monkeypatch.setattr(ops, "adapter_block_bytes", 0 if request.param == "two launches" else 1 << 40)
+        monkeypatch.setattr(ops, "adapter_blocks_bytes", 1 << 40)
+    return request.param
+
+
 MANY = [i % 5 - 1 for i in range(70)]
 PORTIONS = [3] * 40 + [-1] * 30 + [0] * 17 + [2] + [3] + [1] * 90
 
@@ -65,7 +77,7 @@ PORTIONS = [3] * 40 + [-1] * 30 + [0] * 17 + [2] + [3] + [1] * 90
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("ids", [[2], [-1], [0, 0, 3, -1, 2, 1, 1], MANY, PORTIONS], ids=["one", "none", "seven", "singles", "portions"])
 @pytest.mark.parametrize("k,n,rank", [(512, 320, 16), (264, 1000, 8), (100, 37, 3), (1024, 48, 40), (129, 256, 12)])
-def test_rows(dtype, ids, k, n, rank):
+def test_rows(dtype, ids, k, n, rank, way):
     """One row to many, rows without an adapter, adapters that several requests share; widths and ranks of every alignment."""
     case = _case(ids, k, n, rank, 4, dtype=dtype, seed=k + len(ids))
     _check(case)
@@ -75,7 +87,7 @@ def test_rows(dtype, ids, k, n, rank):
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("ids", [[1, 0, 2], MANY, PORTIONS], ids=["three", "singles", "portions"])
 @pytest.mark.parametrize("ends,interleaved", [([64, 80, 96], False), ([100, 101, 400], False), ([17, 300], False), ([320], True), ([1, 2, 3, 4, 5, 6, 7, 333], False)])
-def test_slices(dtype, ids, ends, interleaved):
+def test_slices(dtype, ids, ends, interleaved, way):
     """Stacked projections: slices that end inside a tile, narrow ones, and two that alternate by eights."""
     for rank in (16, 72):
         _check(_case(ids, 256, ends[-1], rank, 4, None if interleaved else ends, dtype, seed=len(ends), interleaved=interleaved))
@@ -83,12 +95,12 @@ def test_slices(dtype, ids, ends, interleaved):
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("ids", [[1, -1, 2], PORTIONS], ids=["three", "portions"])
-def test_residual(dtype, ids):
+def test_residual(dtype, ids, way):
     case = _case(ids, 512, 272, 16, 4, dtype=dtype)
     _check(case, residual=torch.randn(len(ids), 272, generator=torch.Generator().manual_seed(4)))
 
 
-def test_a_row_does_not_hang_on_the_rows_beside_it():
+def test_a_row_does_not_hang_on_the_rows_beside_it(way):
     """Rows of other requests move nothing, whatever they hold; ids outside the slots are rows without an adapter."""
     case = _case(PORTIONS, 512, 320, 16, 4)
     first = _run(case)
@@ -99,7 +111,7 @@ def test_a_row_does_not_hang_on_the_rows_beside_it():
     assert torch.equal(got[1::2], first[1::2]) and bool(torch.isnan(got[::2]).all())
 
 
-def test_streams_and_graphs():
+def test_streams_and_graphs(way):
     from tempura_amd.kernels import ops
     for ids in ([0, 3, -1, 2], PORTIONS):
         s, ends, _ = _case(ids, 512, 320, 16, 4, [128, 320])
@@ -145,7 +157,7 @@ def test_refusals():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_many_adapters_and_long_rows(dtype):
+def test_many_adapters_and_long_rows(dtype, way):
     """More adapters than one pass of the plan takes, most of them with one row; one adapter with rows all over the batch; K in several parts."""
     _check(_case([(i * 37) % 1300 - 1 for i in range(400)], 64, 48, 8, 1299, dtype=dtype))
     _check(_case([0 if i % 3 else (i // 3) % 4 for i in range(700)], 4104, 80, 16, 4, dtype=dtype))

@@ -10,6 +10,13 @@ DEV = "cuda:0"
 BF16, F32 = torch.bfloat16, torch.float32
 
 
+@pytest.fixture(autouse=True)
+def few_keys_too(monkeypatch):
+    """Shared keys are read once for all however few they are (``test_few_shared_keys`` apart)."""
+    from tempura_amd.kernels import ops
+    monkeypatch.setattr(ops, "prefix_least_keys", (0, 0, 0))
+
+
 def _run(s, sink=None, cap=0.0, own=True, dev=DEV):
     from tempura_amd.kernels import ops
     shared = ops.SharedKeys(s["counts"], s["lens"], dev, requests=len(s["new"]))
@@ -85,6 +92,20 @@ def test_other_sizes_run_the_attention_of_each_request():
         to = {name: s[name].to(DEV) for name in ("q", "k", "v", "tables", "starts", "ctx", "req")}
         plain = ops.paged_attention(to["q"], to["k"], to["v"], to["tables"], to["starts"], to["ctx"], to["req"], s["scale"], 0, 1, int(s["ctx"].max()))
         assert torch.equal(_run(s), plain)
+
+
+def test_few_shared_keys(monkeypatch):
+    """By the rule on how many keys are shared: the same bits as without sharing where they are few, the result as defined on both sides."""
+    from tempura_amd.kernels import ops
+    monkeypatch.undo()
+    for dtype, new, below, above in ((BF16, 1, 752, 768), (F32, 1, 496, 512), (BF16, 3, 176, 192), (BF16, 20, 304, 320)):
+        for shared in (below, above):
+            s = P.step([(3, shared)], [20, 30, 41], [new] * 3, 4, 2, 64, 16, dtype, seed=shared)
+            _check(s)
+            to = {name: s[name].to(DEV) for name in ("q", "k", "v", "tables", "starts", "ctx", "req")}
+            plain = ops.paged_attention(to["q"], to["k"], to["v"], to["tables"], to["starts"], to["ctx"], to["req"], s["scale"], 0, new, int(s["ctx"].max()))
+            if shared == below:
+                assert torch.equal(_run(s), plain)
 
 
 def test_large_scores_and_equal_keys():
