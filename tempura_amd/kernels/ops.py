@@ -1607,14 +1607,16 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     _need(softcap >= 0, "prefix_attention: softcap must not be negative")
     # (what a call is refused for by its shapes, and how it is laid out, is found once for calls that are alike; the most own keys rounded up, so that
     # a growing step finds its plan again)
-    key = (q.shape, k_cache.shape, v_cache.shape, block_tables.shape, q.dtype, k_cache.dtype, v_cache.dtype, max_q_len, max_context_len, (own + 255) // 256)
+    key = (q.shape, k_cache.shape, v_cache.shape, block_tables.shape, q.dtype, k_cache.dtype, v_cache.dtype, max_q_len, (own + 255) // 256)
     plan = shared._plans.get(key)
     if plan is None:
-        plan = _prefix_checked(q, k_cache, v_cache, block_tables, shared, int(max_q_len), int(max_context_len), (own + 255) // 256 * 256)
+        plan = _prefix_checked(q, k_cache, v_cache, block_tables, shared, int(max_q_len), (own + 255) // 256 * 256)
         if len(shared._plans) >= 256:
             shared._plans.clear()
         shared._plans[key] = plan
     n, r, heads, sizes, room = plan
+    if not shared.max_keys < max(1, max_context_len) <= block_tables.shape[1] * k_cache.shape[2]:
+        raise KernelError("prefix_attention: the longest context must be longer than the shared keys (new tokens lie behind them) and fit the block table")
     if not (cu_seqlens.dtype == context_lens.dtype == token_req.dtype == block_tables.dtype == torch.int32 and cu_seqlens.numel() > r
             and context_lens.numel() >= r and token_req.numel() >= n):
         raise KernelError("prefix_attention: block_tables, cu_seqlens [r + 1], context_lens [r] and token_req [n] must be int32")
@@ -1633,7 +1635,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
-def _prefix_checked(q, k_cache, v_cache, block_tables, shared: SharedKeys, max_q_len: int, max_context_len: int, own: int) -> tuple:
+def _prefix_checked(q, k_cache, v_cache, block_tables, shared: SharedKeys, max_q_len: int, own: int) -> tuple:
     """(tokens, requests, heads, the kernel's sizes or None where ``paged_attention`` runs, floats of scratch) of calls with these shapes."""
     _need(q.dim() == 3 and k_cache.dim() == 4 and v_cache.dim() == 4, "prefix_attention: bad operand ranks")
     n, heads, d = q.shape
@@ -1647,8 +1649,6 @@ def _prefix_checked(q, k_cache, v_cache, block_tables, shared: SharedKeys, max_q
     if shared.requests != r:
         raise KernelError(f"prefix_attention: runs of {shared.requests} requests for a batch of {r}")
     _need(n >= r and max_q_len >= 1, "prefix_attention: every request brings at least one token")
-    _need(max_context_len <= width * page_size, "prefix_attention: block table narrower than the longest context")
-    _need(shared.max_keys < max(1, max_context_len), "prefix_attention: a request's new tokens must lie behind its shared keys")
     if shared.max_keys == 0 or not prefix_attention_ok(q.dtype, heads, kvh, d, vd, page_size, max_q_len):
         return n, r, heads, None, 0
     least = prefix_least_keys[int(q.dtype == torch.float32)] if max_q_len == 1 else max(prefix_least_keys[2], min(prefix_least_keys[2], 16) * max_q_len)
@@ -1664,42 +1664,49 @@ def _prefix_checked(q, k_cache, v_cache, block_tables, shared: SharedKeys, max_q
     return n, r, heads, (ctypes.c_int * len(sizes))(*sizes), room
 
 
+#: What a launch of ``prefix_attention`` takes (us), by element type: a block's beginning, seen by itself and among others; a block with own keys and a step
+#: of its; a MB of parts joined, and of keys and values read; for blocks of 16, 64 and 128 rows a step of 32 keys of head size 128, of a block by
+#: itself and of one among others on its CU; and with which powers of the head size these two go.  Fitted to 40,000 timed layouts of 881 steps (2 to 100 requests,
+#: 1 to 40 tokens each, 200 to 80,000 shared keys, 4 and 8 key heads of 64 and 128, groups of 1 to 8).  Of 890 other steps the layout that comes
+#: out cheapest takes on average 5 (float32: 7) % longer than the best that was timed, and a tenth of them more than 12 (19) %.
+PREFIX_COSTS = {torch.bfloat16: (0.63, 0.58, 0.115, 0.29, 0.53, 0.086, (0.17, 0.565, 0.68), (0.243, 0.289, 0.335), 0.5, 1.75),
+                torch.float32: (0.9, 0.35, 1.09, 1.2, 1.07, 0.1, (0.36, 1.87, 1.92), (0.43, 0.76, 1.48), 1.2, 1.2)}
+
+
 def _prefix_plan(shared: SharedKeys, r: int, n: int, group: int, kvh: int, max_q_len: int, own: int, dim: int, dtype: torch.dtype) -> tuple:
     """(rows of a block with shared keys, with own keys, blocks of the former a key head and part, steps of 32 keys a part, parts, both for own keys)."""
-    f32 = dtype == torch.float32
-    # Rows: 16, whose keys the waves of a block share out, or 64 and 128, 16 and 32 a wave, which load a step once for all.  (8 requests of 4 heads a
-    # key head behind 2,048 keys: blocks of 16 / 64 rows 12.0 / 11.8 us; 32 behind 65,536: 64 / 128 92 / 75.)
-    most = min(n, shared.max_requests * max_q_len) * group
+    begin, begin_among, own_block, own_step, join, read, step_alone, step_among, power_alone, power_among = PREFIX_COSTS[dtype]
+    f_alone, f_among, size = (dim / 128) ** power_alone, (dim / 128) ** power_among, 4 if dtype == torch.float32 else 2
+    # Rows: 16, whose keys the waves of a block share out, or 64 and 128, 16 and 32 a wave, which load a step once for all.
     own_rows = 16 if max_q_len * group <= 16 else 64 if max_q_len * group <= 64 else 128
-    rows = max(own_rows, 16 if most <= 16 else 64 if most <= 64 else 128)
-    single = max_q_len == 1 and n == r
-    blocks = sum(-(-c * group // rows) for c, _ in shared._runs) if single and not shared._bound else \
-        (n * group - shared.sharing) // rows + shared.sharing
-    own_blocks = r * -(-max_q_len * group // own_rows)
-    # Parts: as long as the launch would take if it were spread evenly, less what a block takes to begin and the join.  A step takes a
-    # block that is alone on its CU step_us, two blocks twice that each; 5.5 TB/s is what single tokens' attention gets from memory.
-    # (64 requests behind 8,192 keys, 600 of their own: parts of 16 / 32 / 43 steps 50.6 / 45.7 / 53.7 us; 32 behind 65,536: 22 / 43 / 64 steps 85 / 75 / 78.)
-    step_us = (0.8 if rows == 128 else 0.55) * dim / 128 * (3 if f32 else 1)
-    slots = 256 if f32 and dim == 128 else 512
-    size = 4 if f32 else 2
-    row_steps = sum(-(-c * n // max(1, r) * group // rows) * -(-v // 32) for c, v in shared._runs) * kvh
+    own_blocks = r * kvh * -(-max_q_len * group // own_rows)
     own_steps = (own + 15 + 31) // 32
-    work_us = (2 * step_us * row_steps + own_blocks * kvh * (4 + own_steps * step_us / 4)) / slots
-    bytes_us = 2 * kvh * dim * size * (sum(v for _, v in shared._runs) + r * own / 2) / 5.5e6
-    steps = -(-shared.max_keys // 32)
-    per = max(8 if rows == 16 else 4, int(0.7 * max(work_us, bytes_us) / step_us))
-    parts = -(-steps // per)
-    # (More than a block a CU and less than one and a half is the worst of both: the CUs with two blocks set the time, 312 blocks 82 us, 384 75.  What is
-    # bound by its arithmetic fills the chip, but never a little more than one round: 56 blocks a part, 10 / 9 / 8 parts 52.5 / 44.0 / 46.0 us.)
-    if blocks * kvh * parts > slots // 2:
-        parts = max(parts, 3 * slots // 4 // (blocks * kvh))
-    if work_us > bytes_us:
-        parts = max(parts, min(-(-steps // 8), slots // (blocks * kvh)))
-    parts = max(1, min(parts, 112, slots // (blocks * kvh)))
-    per = -(-steps // parts)
     # (own keys: two steps a wave, four where there are many blocks; not in more parts than fill the chip a few times, which for portions is one)
-    own_per = max(8 if own_blocks * kvh < 256 else 16, -(-own_steps // max(1, min(16, 2048 // (own_blocks * kvh)))))
-    return rows, own_rows, blocks, per, -(-steps // per), own_per, -(-own_steps // own_per)
+    own_per = max(8 if own_blocks < 256 else 16, -(-own_steps // max(1, min(16, 2048 // own_blocks))))
+    own_parts = -(-own_steps // own_per)
+    own_work = own_block * own_blocks + own_step * own_blocks * own_steps * f_among / 2
+    reading = read * 2e-6 * kvh * dim * size * (sum(v for _, v in shared._runs) + r * own / 2)
+    steps, best = -(-shared.max_keys // 32), None
+    single = max_q_len == 1 and n == r
+    for i, rows in enumerate((16, 64, 128)):
+        if rows < own_rows:
+            continue
+        blocks = sum(-(-c * group // rows) for c, _ in shared._runs) if single and not shared._bound else (n * group - shared.sharing) // rows + shared.sharing
+        runs = [(-(-max(1, round(c * n / max(1, r) * group)) // rows) * kvh, -(-v // 32)) for c, v in shared._runs]
+        work = step_among[i] * f_among * sum(b * s for b, s in runs) + own_work
+        for parts in (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64, 80, 96, 112):
+            if parts > 1 and (parts > steps or blocks * kvh * parts > 6000 or n * group * kvh * (parts + own_parts) * (dim + 2) * 4 > prefix_scratch_limit):
+                break
+            per = -(-steps // parts)
+            of_runs = sum(b * -(-s // per) for b, s in runs)
+            # by itself, a block's longest part; spread over 256 CUs, all blocks' work, and the blocks of the CU that has most
+            alone = max(begin + step_alone[i] * per * f_alone, reading)
+            among = max(max(1, -(-of_runs // 256)) * (begin_among + step_among[i] * per * f_among), (begin_among * of_runs + work) / 256)
+            cost = (alone ** 4 + among ** 4) ** 0.25 + join * 4e-6 * n * group * kvh * (parts + own_parts) * dim
+            if best is None or cost < best[0]:
+                best = (cost, rows, blocks, per)
+    _, rows, blocks, per = best
+    return rows, own_rows, blocks, per, -(-steps // per), own_per, own_parts
 
 
 def swiglu(gu: torch.Tensor, out_dtype: torch.dtype) -> torch.Tensor:
