@@ -4,7 +4,7 @@
 // A group is a run of neighbouring requests of the batch whose block tables begin with the same pages: its first P keys.  Every
 // query of the group sees all of them, so for one key head all (token, head) pairs of the group are the rows of ONE product with
 // those keys, no mask between them; behind them each request has keys of its own, of which its tokens see those up to themselves.
-// A block takes one key head, 16 * NQ rows and one part of the keys (a group's shared ones or a request's own) and leaves the
+// A block takes one key head, 16, 64 or 128 rows and one part of the keys (a group's shared ones or a request's own) and leaves the
 // rows' partial results: O (unnormalised), maximum and sum.  A second kernel joins a row's parts in ascending order:
 //   m = max m_s,   out = sum_s 2^(m_s - m) O_s / (sum_s 2^(m_s - m) l_s + 2^(sink - m)).
 //
@@ -17,9 +17,13 @@
 // Statistics and sums are float32; the probabilities of bfloat16 caches are rounded to bfloat16 for the second product (errors of up to
 // 2^-8 of each, which average out in the sum, itself rounded to bfloat16 at the end).
 //
-// Each of a block's four waves takes a run of the part's steps and has a ring of NB steps in LDS for itself, filled by direct
-// global-to-LDS loads (whole kilobytes) and emptied without a barrier: a step's keys go on their way as soon as the fragments of the
-// keys they replace are in registers, its values likewise.  So every key and value passes a CU's LDS once for up to 64 rows.
+// Two forms of a block of four waves, both fed by direct global-to-LDS loads in whole kilobytes: 16 rows, which every wave takes with a run of
+// the part's steps of its own (prefix_part), and 64 or 128, of which every wave takes a quarter through all steps (prefix_part_rows).  The first asks for
+// the keys once for every 16 rows, from an L2 that has them, but divides a part's steps by four and needs no barrier: best where rows and keys are few
+// for the chip.  32 heads of 128 over 8, requests behind shared keys (16 / 64 / 128 rows a block, each with its best parts, us): 16 behind 2,048
+// 12.7 / 14.2 / 14.9, 32 behind 2,048 14.9 / 17.1 / 19.9, 64 behind 4,096 27.3 / 26.1 / 27.8, 32 behind 16,384 36.3 / 32.9 / 31.6.
+// Bound by: few rows, the trips to memory that a part begins and ends with (8 requests behind 2,048 keys: 12 us for 16 MB); many rows, the rate at which a
+// CU takes a step of one block's products beside another's exponentials (16 requests of up to 24 tokens behind 6,000 keys: 44 us, 440 TFLOP/s).
 #include <math.h>
 
 #include "common.h"
@@ -50,8 +54,8 @@ struct PrefixArgs {
   float* stats;              // [token, head, part, 2]: maximum, sum
   int table_width, page_shift, n_heads, n_kv, groups, requests;
   int single;                // every request brings one token: request r's is token r
-  int shared_blocks;         // blocks (of rows and parts) that take shared keys, a key head each; the own keys' come behind them
-  int shared_rows;           // blocks of rows among them (an upper bound: those beyond the last group end at once)
+  int shared_blocks;         // blocks (of rows and parts) that take shared keys, a key head each; the own keys' come behind them.  An upper
+                             // bound: those beyond the last group end at once
   int own_rows;              // blocks of rows of a request
   int shared_steps, own_steps;   // steps of 32 keys a part has
   int shared_parts, parts;   // a row's places for parts: those of the shared keys, all
@@ -293,7 +297,8 @@ __device__ inline void prefix_queries(const PrefixArgs& a, const PartRows& w, in
 }
 
 // Few rows: every wave takes all of them and a run of the part's steps, through a ring of its own of one step, filled again as soon as its
-// fragments are in registers; no barrier until the waves' sums are added.  (Two blocks a CU: eight steps on their way.)  NT: keys and values are read by one block only.
+// fragments are in registers; no barrier until the waves' sums are added.  (Two blocks a CU: eight steps on their way.)  NT: keys and values are read
+// by one block only.
 template <int E, int D, int NQ, bool NT>
 __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, const PartRows& w, int kvh) {
   using L = PrefixLane<E, D>;
@@ -543,7 +548,7 @@ __device__ inline void prefix_part_rows(const PrefixArgs& a, unsigned char* stag
   }
 }
 
-// How a block takes its rows: KEYS, few of them, 16 * NQ rows whose keys the waves share out; ROWS, 64 * NQ rows, 16 * NQ for a wave.
+// NS 0: 16 * NQ rows whose keys the waves share out; else 64 * NQ rows, 16 * NQ for a wave.
 template <int E, int D, int NQ, int NS, bool NT>
 __device__ inline void prefix_block(const PrefixArgs& a, unsigned char* stages, const PartRows& w, int kvh) {
   if constexpr (NS > 0) prefix_part_rows<E, D, NQ, NS>(a, stages, w, kvh);
@@ -632,7 +637,8 @@ template <int E, int D, int W>
 __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restrict__ sums, const float* __restrict__ stats,
                                                           const int* __restrict__ token_req, const int* __restrict__ context_lens,
                                                           const int* __restrict__ shared_keys, void* __restrict__ out, const float* __restrict__ sink,
-                                                          int rows, int heads, int shared_parts, int parts, int shared_steps, int own_steps, int single) {
+                                                          int rows, int heads, int requests, int shared_parts, int parts, int shared_steps, int own_steps,
+                                                          int single) {
   constexpr int LANES = D / 4, GROUPS = W * 64 / LANES, AHEAD = 4;      // parts at a time, and how many times that is asked for at once
   __shared__ __attribute__((aligned(16))) float red[W > 1 ? W * D : 4];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -644,6 +650,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restric
   if (64 + lane < parts) st[1] = *(const float2*)(s + (64 + lane) * 2);
   const float sunk = sink != nullptr ? sink[row % heads] : 0.f;
   const int r = single ? row / heads : token_req[row / heads];
+  if (r < 0 || r >= requests) return;      // (a row behind the last request: left as it was)
   const int shared = shared_keys[r], ctx = context_lens[r];
   const int n_shared = min(((shared + 31) / 32 + shared_steps - 1) / shared_steps, shared_parts);
   const int n = n_shared + min(((ctx - (shared & ~15) + 31) / 32 + own_steps - 1) / own_steps, parts - shared_parts);
@@ -742,7 +749,7 @@ static int prefix_sizes(const PrefixArgs& a, int blocks, int rows_shared, int ro
 
 // q [n, heads, dim] over pages of keys and transposed values (elements of dt), each request's context by its block table; out [n, heads * dim].
 // groups of requests share their first keys (group_starts [groups + 1], group_keys [groups], shared_keys [requests]: see PrefixArgs); every query
-// lies behind its request's shared keys.  shared_blocks: at least as many blocks of rows_shared rows (16, 64 or 128) as all groups have; rows_own 16, 64 or 128.  Parts of
+// lies behind its request's shared keys; rows of q whose token_req is no request are left as they were.  shared_blocks: at least as many blocks of rows_shared rows (16, 64 or 128) as all groups have; rows_own 16, 64 or 128.  Parts of
 // shared_steps / own_steps steps of 32 keys, as many as there are at most.  scratch: n * heads * (shared_parts + own_parts) * (dim + 2) + 2 floats, aligned to 16 bytes.
 // sizes: element type, table width, n, requests, groups, heads, key heads, dim, page size, the most tokens of a request, rows_shared, rows_own,
 // shared_blocks, shared_steps, shared_parts, own_steps, own_parts.
@@ -757,6 +764,7 @@ extern "C" int tp_prefix_attention(const void* q, const void* k_cache, const voi
   TP_REQUIRE(dt == TP_BF16 || dt == TP_F32, "prefix_attention: unsupported element type");
   TP_REQUIRE(dim == 32 || dim == 64 || dim == 128, "prefix_attention: heads of 32, 64 or 128 elements");
   TP_REQUIRE(page_size >= 16 && (page_size & (page_size - 1)) == 0, "prefix_attention: pages of a power of two from 16 on");
+  TP_REQUIRE(scale > 0.f, "prefix_attention: the scale must be positive");
   TP_REQUIRE(kv_heads > 0 && heads % kv_heads == 0 && groups > 0 && max_q_len > 0, "prefix_attention: bad sizes");
   TP_REQUIRE(shared_steps > 0 && own_steps > 0 && shared_parts > 0 && own_parts > 0 && shared_parts + own_parts <= PA_MAX_PARTS && shared_blocks > 0 && rows_own > 0,
              "prefix_attention: bad parts");
@@ -780,7 +788,6 @@ extern "C" int tp_prefix_attention(const void* q, const void* k_cache, const voi
   a.groups = groups;
   a.requests = requests;
   a.single = n == requests && max_q_len == 1;
-  a.shared_rows = shared_blocks;
   a.shared_parts = shared_parts;
   a.own_rows = (int)(((long)max_q_len * (heads / kv_heads) + rows_own - 1) / rows_own);
   a.shared_steps = shared_steps;
@@ -800,11 +807,11 @@ extern "C" int tp_prefix_attention(const void* q, const void* k_cache, const voi
                                                                                             : prefix_sizes<4, 128>(a, (int)blocks, rows_shared, rows_own, s);
   if (rc != 0) return rc;
   TP_CHECK_LAUNCH("prefix_attention");
-  // (a row of more than eight parts has four waves while the rows are not many: 1,024 rows of 32 parts 13.1 -> see below with one)
+  // (a row of more than eight parts has four waves while the rows are not many: 1,024 rows of 32 parts 6.2 us, with one wave each 13.1)
   const int rows = n * heads;
   const bool wide = a.parts > 8 && rows <= 4096;
 #define PA_JOIN_W(E, D, W) prefix_join_kernel<E, D, W><<<W == 1 ? (rows + 3) / 4 : rows, 256, 0, s>>>(a.sums, a.stats, token_req, context_lens, shared_keys, out, sink, \
-                                                                     rows, heads, shared_parts, a.parts, shared_steps, own_steps, a.single)
+                                                                     rows, heads, requests, shared_parts, a.parts, shared_steps, own_steps, a.single)
 #define PA_JOIN(E, D) (wide ? PA_JOIN_W(E, D, 4) : PA_JOIN_W(E, D, 1))
   if (dt == TP_BF16) {
     if (dim == 32) PA_JOIN(2, 32);

@@ -1583,7 +1583,7 @@ class SharedKeys:
         out[len(merged) + 1: groups + 1] = at
 
 
-def prefix_attention_ok(dtype: torch.dtype, heads: int, kvh: int, dim: int, value_dim: int, page_size: int, max_q_len: int) -> bool:
+def prefix_attention_ok(dtype: torch.dtype, dim: int, value_dim: int, page_size: int) -> bool:
     """Whether ``prefix_attention`` reads shared keys once for all (else it is ``paged_attention``)."""
     return allow_fast_attention and dtype in (torch.bfloat16, torch.float32) and dim == value_dim and dim in (32, 64, 128) and page_size >= 16 \
         and page_size & (page_size - 1) == 0
@@ -1596,7 +1596,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """``paged_attention`` (without a window) of a step whose requests begin with the same keys: the same operands and result, but the pages
     that the requests of a run of ``shared`` have in common are read once for all of them.  Every request's block table names its shared pages
     as well; its new tokens lie behind its shared keys.  ``max_own_len``: the most keys that a request has behind its shared ones, its
-    new tokens among them (a bound, at least the longest; None: ``max_context_len``).  Sizes that the kernel is not built for
+    new tokens among them (a bound, at least the longest; None: ``max_context_len``).  Every row of q belongs to
+    a request, whose index in the batch ``token_req`` gives.  Sizes that the kernel is not built for
     (``prefix_attention_ok``), and steps without shared keys or with few (``prefix_least_keys``), run ``paged_attention``."""
     if _backend is not None:
         return _backend.prefix_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, shared, max_q_len,
@@ -1604,7 +1605,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     _dev_ok(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, sink, shared.starts)
     own = int(max_context_len if max_own_len is None else max_own_len)
     _need(0 < own <= max(1, max_context_len), "prefix_attention: max_own_len must be between 1 and the longest context")
-    _need(softcap >= 0, "prefix_attention: softcap must not be negative")
+    _need(softcap >= 0 and scale > 0, "prefix_attention: softcap must not be negative, the scale must be positive")
     # (what a call is refused for by its shapes, and how it is laid out, is found once for calls that are alike; the most own keys rounded up, so that
     # a growing step finds its plan again)
     key = (q.shape, k_cache.shape, v_cache.shape, block_tables.shape, q.dtype, k_cache.dtype, v_cache.dtype, max_q_len, (own + 255) // 256)
@@ -1649,7 +1650,7 @@ def _prefix_checked(q, k_cache, v_cache, block_tables, shared: SharedKeys, max_q
     if shared.requests != r:
         raise KernelError(f"prefix_attention: runs of {shared.requests} requests for a batch of {r}")
     _need(n >= r and max_q_len >= 1, "prefix_attention: every request brings at least one token")
-    if shared.max_keys == 0 or not prefix_attention_ok(q.dtype, heads, kvh, d, vd, page_size, max_q_len):
+    if shared.max_keys == 0 or not prefix_attention_ok(q.dtype, d, vd, page_size):
         return n, r, heads, None, 0
     least = prefix_least_keys[int(q.dtype == torch.float32)] if max_q_len == 1 else max(prefix_least_keys[2], min(prefix_least_keys[2], 16) * max_q_len)
     many = max_q_len == 1 and sum((c - 1) * v for c, v in shared._runs) >= prefix_least_saved

@@ -180,14 +180,15 @@ def test_shared_keys_refusals(calls, monkeypatch):
     good = dict(q=torch.zeros(3, 4, 64), k=torch.zeros(9, 2, 16, 64), v=torch.zeros(9, 2, 64, 16), t=torch.zeros(3, 6, dtype=torch.int32), cu=i32(0, 1, 2, 3),
                 ctx=i32(70, 71, 72), req=i32(0, 1, 2), shared=ops.SharedKeys([3], [64], "cpu"), max_ctx=72, own=8, sink=None, cap=0.0, q_len=1)
 
-    def call(**kw):
+    def call(scale=0.125, **kw):
         o = {**good, **kw}
-        return ops.prefix_attention(o["q"], o["k"], o["v"], o["t"], o["cu"], o["ctx"], o["req"], 0.125, o["shared"], o["q_len"], o["max_ctx"], max_own_len=o["own"],
+        return ops.prefix_attention(o["q"], o["k"], o["v"], o["t"], o["cu"], o["ctx"], o["req"], scale, o["shared"], o["q_len"], o["max_ctx"], max_own_len=o["own"],
                                     sink=o["sink"], softcap=o["cap"])
     for kw in (dict(shared=ops.SharedKeys([2], [64], "cpu")), dict(shared=ops.SharedKeys([3], [80], "cpu")), dict(max_ctx=97), dict(q=good["q"].bfloat16()),
                dict(q=torch.zeros(4, 3, 64).transpose(0, 1)), dict(k=torch.zeros(9, 3, 16, 64)), dict(v=torch.zeros(9, 2, 16, 64)), dict(own=0), dict(own=73),
                dict(sink=torch.zeros(3)), dict(cap=-1.0), dict(ctx=good["ctx"].long()), dict(cu=i32(0, 1, 2)), dict(req=i32(0, 1)), dict(t=good["t"][0]),
-               dict(q=torch.zeros(2, 4, 64)), dict(q_len=0), dict(t=good["t"].long())):
+               dict(q=torch.zeros(2, 4, 64)), dict(q_len=0), dict(t=good["t"].long()), dict(scale=0.0),
+               dict(scale=-1.0), dict(max_ctx=64)):
         with pytest.raises(KernelError):
             call(**kw)
     assert not calls
