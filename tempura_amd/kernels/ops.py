@@ -897,14 +897,15 @@ ADAPTER_SLICES = 8
 #: rows are taken one by one up to this many, single tokens up to that many,
 adapter_row_limits = (256, 512)
 #: where no more than so many bytes of adapters' weights are read that way, and so many more for each adapter that single tokens may have; else
-#: rows with the same adapter are taken together.  (us beside the shared product, rank x K, 4,096 columns, bf16, one by one / together: 128 rows of
-#: 4 adapters, 32 x 4,096 10.5 / 11.9, 64 x 4,096 19.4 / 12.9, 16 x 14,336 12.0 / 14.4, 32 x 14,336 19.9 / 15.0; 192 rows, 32 x 1,024 11.7 / 10.8, 16 x 4,096
-#: 10.1 / 12.1.  Of
+#: rows with the same adapter are taken together.  (us beside the shared product, rank x K, one by one / together, rows of 4 adapters; bf16, 4,096 columns: 128
+#: rows of 32 x 4,096, 64 MB, 10.5 / 11.9, 64 x 4,096, 134 MB, 19.4 / 12.9; of three slices of 16 x 4,096 70 rows, 35 MB, 9.0 / 15.1, of 64 x 1,024 104 MB,
+#: 19.1 / 13.6; float32: 128 rows of 64 x 4,096, 200 MB, 21.7 / 21.1, 70 of 64 x 8,192, 184 MB, 24.5 / 30.4, 256 of 64 x 8,192, 58 / 34.  Single tokens of
 #: 32 adapters, which then share a window of 64 rows: 128 rows of 64 x 4,096 31 / 39, 256 57 / 58, 512 99 / 93.)
-adapter_row_weights, adapter_row_weights_each = 64 << 20, 8 << 20
+adapter_row_weights, adapter_row_weights_each = {torch.bfloat16: 88 << 20, torch.float32: 224 << 20}, 8 << 20
 #: rows one by one: a launch works their low-rank values out in front where one block would read more than this of A for its row, or all blocks
-#: more than that.  (One launch / two, 16 rows, rank x K: 16 x 4,096 6.0 / 6.7 us, 16 x 8,192 8.0 / 8.1, 64 x 4,096 11.7 / 8.6, 16 x 14,336 11 / 10;
-#: 8 x 4,096 in 768 blocks, 50 MB, 9.1 / 9.5, in 2,048, 134 MB, 18.1 / 16.1, 16 x 4,096 in 512, 67 MB, 9.0 / 8.5.)
+#: more than that (half and a quarter of it where rows are not aligned to 16 bytes).  (One launch / two, 16 rows, rank x K: 16 x 4,096 6.0 / 6.7 us, 16 x 8,192
+#: 8.0 / 8.1, 64 x 4,096 11.7 / 8.6, 16 x 14,336 11 / 10; 8 x 4,096 in 768 blocks, 50 MB, 9.1 / 9.5, in 2,048, 134 MB, 18.1 / 16.1, 16 x 4,096 in 512, 67 MB,
+#: 9.0 / 8.5; not aligned, 16 x 1,100 of 64 rows, 9 MB, 6.2 / 7.0, of 128 10.0 / 8.5, 64 x 1,100 8.2 / 7.1.)
 adapter_block_bytes, adapter_blocks_bytes = 192 << 10, 48 << 20
 
 
@@ -965,9 +966,12 @@ def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, re
         return linear(x, w, torch.float32, residual=residual)
     # (single tokens by the rows that a captured step of as many has, for the same bits)
     rows, ranks, size = decode_rows_padded(m) if max_run == 1 else m, adapters.slices * adapters.rank, x.element_size()
-    most = adapter_row_weights + (adapter_row_weights_each * min(adapters.slots, 64) if max_run == 1 else 0)
+    most = adapter_row_weights[adapters.dtype] + (adapter_row_weights_each * min(adapters.slots, 64) if max_run == 1 else 0)
     if rows <= adapter_row_limits[max_run == 1] and rows * (ranks * k + adapters.rank * adapters.n) * size <= most:
-        two = adapters.rank * k * size > adapter_block_bytes or rows * -(-adapters.n // 1024) * adapters.rank * k * size > adapter_blocks_bytes
+        # (a block of 1,024 columns reads the A of each slice that they lie in)
+        blocks, of_slice, aligned = -(-adapters.n // 1024), adapters.rank * k * size, _adapter_rows_aligned(x, adapters)
+        of_slices = blocks * 2 if adapters.interleaved else blocks + adapters.slices - 1
+        two = of_slice * (1 if aligned else 2) > adapter_block_bytes or rows * of_slices * of_slice * (1 if aligned else 4) > adapter_blocks_bytes
         y = linear(x, w, torch.float32, residual=residual)
         _adapter_add(x, adapters, ids, y, 0, 0, two)
         return y
@@ -979,11 +983,15 @@ def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, re
     return linear(x, w, torch.float32, residual=y)
 
 
+def _adapter_rows_aligned(x: torch.Tensor, adapters: Adapters) -> bool:
+    return x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0 and adapters.a.data_ptr() % 16 == 0
+
+
 def _adapter_add(x: torch.Tensor, adapters: Adapters, ids: torch.Tensor, y: torch.Tensor, parts: int, write: int, two: bool = False) -> None:
     m, k = x.shape
     _need(y.dtype == torch.float32 and tuple(y.shape) == (m, adapters.n), "adapter_linear: residual must be float32 [m, n]")
     scratch = torch.empty((max(parts, 1) * m * adapters.slices * adapters.rank,), dtype=torch.float32, device=x.device) if parts or two else None
-    vec = int(k % 8 == 0 and x.data_ptr() % 16 == 0 and adapters.a.data_ptr() % 16 == 0)
+    vec = int(_adapter_rows_aligned(x, adapters))
     _call("tp_adapter_add", _ptr(ids), _ptr(x), _dt(x), _ptr(adapters.a), _ptr(adapters.b), _ptr(adapters.scales), _ptr(y), m, k, adapters.n,
           adapters.slots, adapters.rank, adapters.slices, int(adapters.interleaved), adapters.ends, vec, parts, write, _ptr(scratch), _stream(),
           tag=(m, adapters.n, k))
@@ -1490,12 +1498,12 @@ def attention_rows(rows, col0: int, ctx, group: int, heads: int, kvh: int, dim: 
 
 #: the engine's steps of single tokens, and of portions of up to 128, read shared keys once for all where that saves at least so many bytes of keys and
 #: values a layer; of longer portions as many times more as they are longer, of portions up to 64 a twelfth.  (Single tokens behind shared keys, 32 heads of
-#: 128 over 8 key heads, bf16, a layer of a captured step, once for all / each for itself, the projections and ``attention_rows``' own work among it:
-#: 2 requests of 8,192 keys, 34 MB, 138 / 135 us; 4 of 4,096, 50 MB, 135 / 135; 8 of 2,048, 59 MB, 137 / 138; 32 of 1,024, 130 MB, 174 / 169;
-#: 32 of 2,048, 260 MB, 174 / 175; 64 of 1,024, 264 MB, 182 / 186; 8 of 8,192, 235 MB, 143 / 153; 32 of 8,192, 1,040 MB, 183 / 215.  The attention alone of
+#: 128 over 8 key heads, bf16, a captured step of four layers with embedding and head, us, once for all / each for itself: 2 requests of 8,192 keys,
+#: 34 MB a layer saved, 545 / 542; 4 of 4,096, 50 MB, 541 / 542; 8 of 2,048, 59 MB, 550 / 553; 16 of 2,048, 126 MB, 629 / 648; 32 of 1,024, 130 MB, 685 / 678;
+#: 8 of 8,192, 235 MB, 570 / 613; 32 of 2,048, 260 MB, 692 / 703; 32 of 8,192, 1,040 MB, 732 / 865; 64 of 8,192, 2,110 MB, 784 / 1,206.  The attention alone of
 #: 4 and 32 tokens behind 2,048 or 8,192 keys beside a prompt of its own: 4 x 2,048 and 64 tokens, 25 MB, 17.7 / 23.0; 4 x 8,192 and 512, 100 MB, 80 / 56;
 #: 32 x 8,192 and 512, 91 / 112, and 2,048, 258 / 152.)
-shared_keys_pay_bytes = 192 << 20
+shared_keys_pay_bytes = 96 << 20
 
 
 def shared_keys_pay(saved_bytes: int, longest: int) -> bool:

@@ -64,7 +64,7 @@ def way(request, monkeypatch):
     from tempura_amd.kernels import ops
     if request.param != "rule":
         monkeypatch.setattr(ops, "adapter_row_limits", (0, 0) if request.param == "together" else (1 << 16, 1 << 16))
-        monkeypatch.setattr(ops, "adapter_row_weights", 1 << 40)
+        monkeypatch.setattr(ops, "adapter_row_weights", {BF16: 1 << 40, F32: 1 << 40})
         monkeypatch.setattr(ops, "adapter_block_bytes", 0 if request.param == "two launches" else 1 << 40)
         monkeypatch.setattr(ops, "adapter_blocks_bytes", 1 << 40)
     return request.param
