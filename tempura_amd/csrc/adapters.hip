@@ -202,7 +202,7 @@ __device__ inline void mfma_piece(const ad_u32x4& a, const ad_u32x4& b, ad_f32x4
 
 // v[part, row, ranks] = A x over one part of K, 16 * RT ranks a block: v^T[rank, row] = A[rank, :] . x[row, :]^T.
 // grid: (windows, parts, blocks of ranks * each), a block taking every each-th adapter of its window (the first adapters' blocks in front: those that find
-// none would else take places between the others in the round in which blocks are handed to the CUs).
+// none would else take places between the others in the turn in which blocks are handed to the CUs).
 // This form loads fragments straight into registers, the four waves taking every fourth step, added in LDS in their order: for rows whose length is no
 // multiple of 128 bytes (VEC: but of eight elements) or that are not aligned.
 template <typename T, int RT, bool VEC>
@@ -390,7 +390,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a, const fl
     for (int s = s0; s <= s1; ++s) {
       const int from = a.interleaved ? w0 : max(w0, s > 0 ? a.ends[s - 1] : 0), to = a.interleaved ? w1 : min(w1, a.ends[s]);     // this wave's columns
       for (int j0 = 0; j0 < a.rank; j0 += CHUNK) {
-        const bool add = !write || j0 > 0 || (a.interleaved && s > 0);
+        const bool add = !write || j0 > 0;
         ad_u32x4 bf[CT][STEPS];
 #pragma unroll
         for (int i = 0; i < CT; ++i) {
@@ -471,7 +471,8 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a, const fl
 #pragma unroll
           for (int i = 0; i < 16 / ROWS; ++i) {
             const int row = i * ROWS + lane / LANES, col = lane % LANES * 4;
-            if (t * 16 + row >= count) continue;
+            // (another slice's columns between this one's: zero times these low-rank values, no numbers where the values are infinite)
+            if (t * 16 + row >= count || (a.interleaved && (((w0 + col) >> 3) & 1) != s)) continue;
             ad_f32x4 value = *(const ad_f32x4*)(tile[wave] + row * OUT + col);
             float* y = a.y + (size_t)order[t * 16 + row] * a.N + w0 + col;
             if (VEC && w0 + col >= from && w0 + col + 4 <= to) {

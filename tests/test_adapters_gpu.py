@@ -111,6 +111,23 @@ def test_a_row_does_not_hang_on_the_rows_beside_it(way):
     assert torch.equal(got[1::2], first[1::2]) and bool(torch.isnan(got[::2]).all())
 
 
+@pytest.mark.parametrize("ids", [[1, -1, 2], PORTIONS], ids=["three", "portions"])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("ends,interleaved", [([320], True), ([100, 320], False)])
+def test_a_slice_that_is_not_finite_leaves_the_others(ids, dtype, ends, interleaved, way):
+    """Low-rank values of one slice that are infinite or no numbers: the other slice's columns, beside or between its own, are as without it."""
+    from tempura_amd.kernels import ops
+    case = _case(ids, 256, 320, 16, 4, None if interleaved else ends, dtype, seed=3, interleaved=interleaved)
+    want, tol = _exact(*case)
+    col = torch.arange(320)
+    other = (col // 8) % 2 == 1 if interleaved else col >= 100
+    case[0]["a"][:, :16] = float("inf")
+    got = _run(case).cpu().double()
+    assert float(((got - want).abs() - tol)[:, other].max()) <= 0
+    some = case[0]["ids"] >= 0
+    assert not bool(torch.isfinite(got[some][:, ~other]).any()) and bool(torch.isfinite(got[~some]).all())
+
+
 def test_streams_and_graphs(way):
     from tempura_amd.kernels import ops
     for ids in ([0, 3, -1, 2], PORTIONS):
