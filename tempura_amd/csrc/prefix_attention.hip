@@ -569,7 +569,7 @@ __global__ __launch_bounds__(PA_WAVES * 64, OCC) void prefix_attention_kernel(Pr
     // which group's rows: a lane counts the blocks of one group, 64 groups at a time
     const int lane = threadIdx.x & 63;
     // (a group's blocks of rows one behind the other, so that those that are not there come last: between the others they would take places
-    // of the round in which the blocks are handed to the CUs)
+    // of the first turn in which blocks are handed to the CUs)
     int rb = b / a.shared_parts;
     w.part = b % a.shared_parts;
     bool found = false;

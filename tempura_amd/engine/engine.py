@@ -180,7 +180,7 @@ class Engine:
         if self._ahead is not None:      # a queued step's logits live in a graph's output buffer: keep a copy
             self._ahead = (self._ahead[0], ops.take_rows(self._ahead[1]))
         handle = next(self._own_ids)
-        rid = ("prefix", handle)
+        rid = ("prefix", handle, object())      # (no request's id, whatever the caller names those)
         self.runner.add_request(rid)
         if adapter is not None:
             self.runner.adapter_of[rid] = self._adapters[adapter]

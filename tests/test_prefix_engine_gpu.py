@@ -47,6 +47,11 @@ def test_tokens_are_those_of_whole_prompts(tiny_dirs, always, name, kw):
     for _ in range(4):
         eng.step()
     eng.release_prefix(b)
+    late = eng.hold_prefix(two + one)      # (between steps of others, one of them queued ahead)
+    eng.step()
+    tails.append(tails[0])
+    which.append((late, two + one))
+    lengths.append(5)
     rids += [eng.add_request(t, SamplingParams(temperature=0.0, max_new_tokens=n), prefix=p) for t, (p, _), n in zip(tails[6:], which[6:], lengths[6:])]
     while eng.has_unfinished():
         eng.step()
@@ -54,6 +59,7 @@ def test_tokens_are_those_of_whole_prompts(tiny_dirs, always, name, kw):
         assert eng.request(rid).output == plain.greedy_generate(cfg, W, tokens + t, n)
     assert always and (eng.stats()["graph_steps"] > 0) == kw.get("use_graph", True)
     eng.release_prefix(a)
+    eng.release_prefix(late)
     assert eng.runner.cache.free_pages() == [128]
 
 
