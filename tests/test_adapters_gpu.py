@@ -128,6 +128,11 @@ def test_a_slice_that_is_not_finite_leaves_the_others(ids, dtype, ends, interlea
     assert not bool(torch.isfinite(got[some][:, ~other]).any()) and bool(torch.isfinite(got[~some]).all())
 
 
+def test_no_rows():
+    case = _case([], 64, 48, 8, 2)
+    assert _run(case).shape == (0, 48) and _run(case, residual=torch.empty(0, 48, device=DEV), max_run=1).shape == (0, 48)
+
+
 def test_streams_and_graphs(way):
     from tempura_amd.kernels import ops
     for ids in ([0, 3, -1, 2], PORTIONS):

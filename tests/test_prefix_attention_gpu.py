@@ -181,8 +181,32 @@ def test_runs_of_a_captured_step_move_between_replays(dtype):
         assert bool(torch.isfinite(out).all()) and float(over.max()) <= 0, float(over.max())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_pages_beyond_two_to_the_31_elements(dtype):
+    """The same step at the far end of a pool of more than 2^31 elements (and 2^32 bytes): the same bits."""
+    s = P.step([(6, 512), (2, 0)], [1 + 41 * i for i in range(8)], [1] * 7 + [5], 8, 2, 128, 16, dtype, seed=9, poison=False)
+    near = _run(s)
+    pages, first = s["k"].shape[0], 2 ** 31 // (2 * 16 * 128) + 7
+    assert (first + pages) * 2 * 16 * 128 > 2 ** 31
+    from tempura_amd.kernels import ops
+    k = torch.empty((first + pages,) + s["k"].shape[1:], dtype=dtype, device=DEV)
+    v = torch.empty((first + pages,) + s["v"].shape[1:], dtype=dtype, device=DEV)
+    k[first:], v[first:] = s["k"].to(DEV), s["v"].to(DEV)
+    t = {name: s[name].to(DEV) for name in ("q", "tables", "starts", "ctx", "req")}
+    tables = torch.where(t["tables"] >= 0, t["tables"] + first, t["tables"])
+    shared = ops.SharedKeys(s["counts"], s["lens"], DEV)
+    far = ops.prefix_attention(t["q"], k, v, tables, t["starts"], t["ctx"], t["req"], s["scale"], shared, 5, int(s["ctx"].max()), max_own_len=s["own"])
+    assert torch.equal(near, far)
+
+
 def test_tokens_that_are_not_there_are_not_written():
-    """No tokens: nothing is launched.  A step's outputs are its own: the scratch of one call does not reach the next."""
+    """No requests: an empty result.  A step's outputs are its own: the scratch of one call does not reach the next."""
+    from tempura_amd.kernels import ops
+    none = lambda *shape: torch.empty(shape, dtype=torch.int32, device=DEV)  # noqa: E731
+    cache = torch.zeros(3, 2, 16, 64, dtype=BF16, device=DEV)
+    out = ops.prefix_attention(torch.empty(0, 4, 64, dtype=BF16, device=DEV), cache, cache.transpose(2, 3).contiguous(), none(0, 1), none(1).zero_(), none(0), none(0), 0.125,
+                               ops.SharedKeys([], [], DEV), 1, 1)
+    assert out.shape == (0, 256)
     s = P.step([(3, 64)], [5, 6, 7], [1, 1, 1], 4, 2, 64, 16, BF16, seed=1)
     a, b = _run(s), _run(s)
     assert a.data_ptr() != b.data_ptr() and torch.equal(a, b)
