@@ -1682,6 +1682,10 @@ PREFIX_COSTS = {torch.bfloat16: (0.63, 0.58, 0.115, 0.29, 0.53, 0.086, (0.17, 0.
                 torch.float32: (0.9, 0.35, 1.09, 1.2, 1.07, 0.1, (0.36, 1.87, 1.92), (0.43, 0.76, 1.48), 1.2, 1.2)}
 
 
+#: into how many parts shared keys are cut: few enough that a row's parts fit the joining kernel beside 16 of own keys
+PREFIX_PARTS = (112, 96, 80, 64, 48, 40, 32, 28, 24, 20, 16, 14, 12, 10, 9, 8, 7, 6, 5, 4, 3, 2, 1)
+
+
 def _prefix_plan(shared: SharedKeys, r: int, n: int, group: int, kvh: int, max_q_len: int, own: int, dim: int, dtype: torch.dtype) -> tuple:
     """(rows of a block with shared keys, with own keys, blocks of the former a key head and part, steps of 32 keys a part, parts, both for own keys)."""
     begin, begin_among, own_block, own_step, join, read, step_alone, step_among, power_alone, power_among = PREFIX_COSTS[dtype]
@@ -1703,15 +1707,19 @@ def _prefix_plan(shared: SharedKeys, r: int, n: int, group: int, kvh: int, max_q
         blocks = sum(-(-c * group // rows) for c, _ in shared._runs) if single and not shared._bound else (n * group - shared.sharing) // rows + shared.sharing
         runs = [(-(-max(1, round(c * n / max(1, r) * group)) // rows) * kvh, -(-v // 32)) for c, v in shared._runs]
         work = step_among[i] * f_among * sum(b * s for b, s in runs) + own_work
-        for parts in (1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 12, 14, 16, 20, 24, 28, 32, 40, 48, 64, 80, 96, 112):
-            if parts > 1 and (parts > steps or blocks * kvh * parts > 6000 or n * group * kvh * (parts + own_parts) * (dim + 2) * 4 > prefix_scratch_limit):
-                break
+        # (from many parts to few, until the longest part alone takes longer than the best layout, beside what all of them take)
+        most = min(steps, 6000 // (blocks * kvh) if blocks else 1, prefix_scratch_limit // (4 * n * group * kvh * (dim + 2)) - own_parts)
+        for parts in PREFIX_PARTS:
+            if parts > most and parts > 1:
+                continue
             per = -(-steps // parts)
-            of_runs = sum(b * -(-s // per) for b, s in runs)
+            alone = begin + step_alone[i] * per * f_alone
+            if best is not None and alone ** 4 + (work / 256) ** 4 > best[0] ** 4:
+                break
             # by itself, a block's longest part; spread over 256 CUs, all blocks' work, and the blocks of the CU that has most
-            alone = max(begin + step_alone[i] * per * f_alone, reading)
+            of_runs = sum([b * -(-s // per) for b, s in runs])
             among = max(max(1, -(-of_runs // 256)) * (begin_among + step_among[i] * per * f_among), (begin_among * of_runs + work) / 256)
-            cost = (alone ** 4 + among ** 4) ** 0.25 + join * 4e-6 * n * group * kvh * (parts + own_parts) * dim
+            cost = (max(alone, reading) ** 4 + among ** 4) ** 0.25 + join * 4e-6 * n * group * kvh * (parts + own_parts) * dim
             if best is None or cost < best[0]:
                 best = (cost, rows, blocks, per)
     _, rows, blocks, per = best
