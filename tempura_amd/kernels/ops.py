@@ -182,6 +182,17 @@ def _dev_ok(*ts) -> None:
                 raise KernelError("operand is not contiguous")
 
 
+def _here_ok(*ts) -> None:
+    """``_dev_ok``, and operands of another device than the current one, whose stream a launch goes to, are refused."""
+    here = torch.cuda.current_device()
+    for t in ts:
+        if t is not None:
+            if t.get_device() != here:
+                raise KernelError("operand is not on the current device")
+            if not t.is_contiguous():
+                raise KernelError("operand is not contiguous")
+
+
 def _i32(t: torch.Tensor, n: int, what: str) -> None:
     if not (t.dtype == torch.int32 and t.numel() >= n and t.dim() >= 1):
         raise KernelError(f"{what}: need int32 with {n} elements")
@@ -942,6 +953,9 @@ class Adapters:
             wide[:, :, :rank] = b
             b = wide
         self.a, self.b, self.scales = a, b, scales
+        # (a block of 1,024 columns reads the A of each slice that they lie in)
+        starts = [0] + ends[:-1]
+        self.slice_blocks = 2 * -(-self.n // 1024) if interleaved else sum((e - 1) // 1024 - b // 1024 + 1 for b, e in zip(starts, ends))
         self.ends = (ctypes.c_int * self.slices)(*(ends if not interleaved else [self.n, self.n]))
 
     @property
@@ -955,23 +969,20 @@ def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, re
     ``max_run``: the most tokens that a request brings (0: not known)."""
     if _backend is not None:
         return _backend.adapter_linear(x, w, adapters, ids, residual)
-    _dev_ok(x, ids, residual)
+    _here_ok(x, ids, adapters.a, residual)
     _need(x.dim() == 2 and x.dtype == adapters.dtype, "adapter_linear: x must be [m, k] of the adapters' type")
     m, k = x.shape
     if not (k == adapters.k and w.dim() == 2 and tuple(w.shape) == (adapters.n, k)):
         raise KernelError(f"adapter_linear: shapes {(m, k)} x {tuple(w.shape)} with adapters of {adapters.k} x {adapters.n}")
     _need(ids.dtype == torch.int32 and ids.dim() == 1 and ids.numel() == m, "adapter_linear: ids must be int32 [m]")
-    _need(x.device == ids.device == adapters.a.device, "adapter_linear: operands on different devices")
     if m == 0:
         return linear(x, w, torch.float32, residual=residual)
     # (single tokens by the rows that a captured step of as many has, for the same bits)
     rows, ranks, size = decode_rows_padded(m) if max_run == 1 else m, adapters.slices * adapters.rank, x.element_size()
     most = adapter_row_weights[adapters.dtype] + (adapter_row_weights_each * min(adapters.slots, 64) if max_run == 1 else 0)
     if rows <= adapter_row_limits[max_run == 1] and rows * (ranks * k + adapters.rank * adapters.n) * size <= most:
-        # (a block of 1,024 columns reads the A of each slice that they lie in)
-        blocks, of_slice, aligned = -(-adapters.n // 1024), adapters.rank * k * size, _adapter_rows_aligned(x, adapters)
-        of_slices = blocks * 2 if adapters.interleaved else blocks + adapters.slices - 1
-        two = of_slice * (1 if aligned else 2) > adapter_block_bytes or rows * of_slices * of_slice * (1 if aligned else 4) > adapter_blocks_bytes
+        of_slice, aligned = adapters.rank * k * size, k % 8 == 0 and x.data_ptr() % 16 == 0
+        two = of_slice * (1 if aligned else 2) > adapter_block_bytes or rows * adapters.slice_blocks * of_slice * (1 if aligned else 4) > adapter_blocks_bytes
         y = linear(x, w, torch.float32, residual=residual)
         _adapter_add(x, adapters, ids, y, 0, 0, two)
         return y
@@ -983,16 +994,14 @@ def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, re
     return linear(x, w, torch.float32, residual=y)
 
 
-def _adapter_rows_aligned(x: torch.Tensor, adapters: Adapters) -> bool:
-    return x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0 and adapters.a.data_ptr() % 16 == 0
-
-
 def _adapter_add(x: torch.Tensor, adapters: Adapters, ids: torch.Tensor, y: torch.Tensor, parts: int, write: int, two: bool = False) -> None:
     m, k = x.shape
-    _need(y.dtype == torch.float32 and tuple(y.shape) == (m, adapters.n), "adapter_linear: residual must be float32 [m, n]")
-    scratch = torch.empty((max(parts, 1) * m * adapters.slices * adapters.rank,), dtype=torch.float32, device=x.device) if parts or two else None
-    vec = int(_adapter_rows_aligned(x, adapters))
-    _call("tp_adapter_add", _ptr(ids), _ptr(x), _dt(x), _ptr(adapters.a), _ptr(adapters.b), _ptr(adapters.scales), _ptr(y), m, k, adapters.n,
+    if y.dtype != torch.float32 or y.shape != (m, adapters.n):
+        raise KernelError("adapter_linear: residual must be float32 [m, n]")
+    scratch = torch.empty(max(parts, 1) * m * adapters.slices * adapters.rank, dtype=torch.float32, device=x.device) if parts or two else None
+    a = adapters.a.data_ptr()
+    vec = int(k % 8 == 0 and x.data_ptr() % 16 == 0 and a % 16 == 0)
+    _call("tp_adapter_add", ids.data_ptr(), x.data_ptr(), _dt(x), a, adapters.b.data_ptr(), adapters.scales.data_ptr(), y.data_ptr(), m, k, adapters.n,
           adapters.slots, adapters.rank, adapters.slices, int(adapters.interleaved), adapters.ends, vec, parts, write, _ptr(scratch), _stream(),
           tag=(m, adapters.n, k))
 
@@ -1610,7 +1619,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if _backend is not None:
         return _backend.prefix_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, shared, max_q_len,
                                          max_context_len, max_own_len, num_single, sink, softcap)
-    _dev_ok(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, sink, shared.starts)
+    _here_ok(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, sink, shared.starts)
     own = int(max_context_len if max_own_len is None else max_own_len)
     _need(0 < own <= max(1, max_context_len), "prefix_attention: max_own_len must be between 1 and the longest context")
     _need(softcap >= 0 and scale > 0, "prefix_attention: softcap must not be negative, the scale must be positive")
@@ -1634,10 +1643,10 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if sizes is None:
         return paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, 0, max_q_len, max_context_len,
                                num_single, sink=sink, softcap=softcap)
-    out = torch.empty((n, heads * q.shape[2]), dtype=q.dtype, device=q.device)
+    out = q.new_empty((n, heads * q.shape[2]))
     if n == 0:
         return out
-    scratch = torch.empty((room,), dtype=torch.float32, device=q.device)
+    scratch = torch.empty(room, dtype=torch.float32, device=q.device)
     _call("tp_prefix_attention", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(), cu_seqlens.data_ptr(), context_lens.data_ptr(),
           token_req.data_ptr(), shared.starts.data_ptr(), shared.keys.data_ptr(), shared.each.data_ptr(), out.data_ptr(), scratch.data_ptr(), _ptr(sink),
           sizes, scale, softcap, _stream())

@@ -145,6 +145,7 @@ def calls(monkeypatch):
     monkeypatch.setattr(ops, "_dev_ok", lambda *ts: [ops._need(t is None or t.is_contiguous(), "operand is not contiguous") for t in ts])
     monkeypatch.setattr(ops, "_call", lambda name, *args, tag=None: made.append((name, args)))
     monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)      # (what host tensors name as theirs)
     monkeypatch.setattr(ops, "linear", lambda x, w, dt, residual=None, **kw: residual if residual is not None else torch.zeros(x.shape[0], w.shape[0]))
     return made
 
@@ -168,6 +169,10 @@ def test_adapter_refusals(calls):
     ops.adapter_linear(x, w, ad, ids)
     ops.adapter_linear(torch.zeros(0, 64), w, ad, ids[:0])
     assert [c[0] for c in calls] == ["tp_adapter_add"]
+    with pytest.MonkeyPatch.context() as mp:
+        mp.setattr(torch.cuda, "current_device", lambda: 1)
+        with pytest.raises(KernelError, match="current device"):
+            ops.adapter_linear(x, w, ad, ids)
     wide = ops.Adapters(torch.zeros(2, 6, 64), torch.zeros(2, 48, 3), sc[:2], [10, 48])      # (ranks padded once)
     assert wide.rank == 8 and tuple(wide.a.shape) == (2, 16, 64) and tuple(wide.b.shape) == (2, 48, 8)
 
@@ -195,6 +200,9 @@ def test_shared_keys_refusals(calls, monkeypatch):
     call()
     call(own=None)
     assert [c[0] for c in calls] == ["tp_prefix_attention"] * 2
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    with pytest.raises(KernelError, match="current device"):
+        call()
     for counts, lens in (([1], [1, 2]), ([-1], [3]), ([1], [-3]), ([1], [2 ** 31])):
         with pytest.raises(KernelError):
             ops.SharedKeys(counts, lens, "cpu")
