@@ -989,7 +989,11 @@ def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, re
     # (many rows: the adapters' share first, onto which the shared product adds its own: it reads y in its epilogue, 118.4 -> 124.0 us for 4,096
     # rows of 4,096 x 4,096 and nothing for 731 of 8,192 x 2,048, where the other order reads it in a pass of its own, 17 us)
     y = torch.empty((m, adapters.n), dtype=torch.float32, device=x.device) if residual is None else residual
-    parts = max(1, min(8, k // 512, 256 // (-(-rows // 64) * -(-ranks // 64))))
+    # Parts of K: float32 256 elements each, bfloat16 512 up to four and 1,024 beyond, as long as blocks are few.  (Rank 16, 2,048 columns, us, 1 / 2 / 4 / 8:
+    # bf16 700 rows of 1,024 12.7 / 11.7 / 11.9 / 12.0, of 2,048 15.1 / 13.1 / 12.5 / 13.3, of 4,096 20.1 / 15.5 / 13.8 / 13.9, 3,000 of 4,096 27.6 / 23.4 / 24.9 / 27.1;
+    # float32 700 of 1,024 18.7 / 14.8 / 13.3 / 13.5, of 4,096 41.7 / 26.6 / 19.5 / 16.7, 3,000 of 4,096 49.3 / 34.9 / 34.4 / 32.2.)
+    blocks = -(-rows // 64) * -(-ranks // 64)
+    parts = max(1, min(8, k // 256, 256 // blocks) if size == 4 else min(8, max(k // 1024, min(4, k // 512)), 128 // blocks))
     _adapter_add(x, adapters, ids, y, parts, int(residual is None))
     return linear(x, w, torch.float32, residual=y)
 
