@@ -353,9 +353,9 @@ class Engine:
         return queue
 
     def generate(self, prompts: Sequence[Sequence[int]], params: Union[SamplingParams, Sequence[SamplingParams], None] = None,
-                 adapters: Union[str, Sequence[Optional[str]], None] = None) -> List[List[int]]:
+                 adapters: Union[str, Sequence[Optional[str]], None] = None, prefix: Optional[int] = None) -> List[List[int]]:
         """Generate for every prompt (token ids in, token ids out); continuous batching inside.  ``adapters``: a loaded adapter's name
-        for all prompts, or one (or None) for each."""
+        for all prompts, or one (or None) for each.  ``prefix``: a handle of ``hold_prefix`` that every prompt comes behind."""
         if params is None or isinstance(params, SamplingParams):
             params = [params or SamplingParams()] * len(prompts)
         if len(params) != len(prompts):
@@ -366,7 +366,9 @@ class Engine:
         for name in names:
             if name is not None and name not in self._adapters:
                 raise ValueError(f"adapter {name!r} is not loaded (loaded: {sorted(self._adapters)})")
-        rids = [self.add_request(p, sp, adapter=a) for p, sp, a in zip(prompts, params, names)]
+        if prefix is not None and (prefix not in self._prefixes or any(name != self._prefixes[prefix][3] for name in names)):
+            raise ValueError(f"prefix {prefix!r} is not held, or was computed with another adapter than a prompt names")
+        rids = [self.add_request(p, sp, adapter=a, prefix=prefix) for p, sp, a in zip(prompts, params, names)]
         while self.has_unfinished():
             self.step()
         return [list(self._requests[r].output) for r in rids]

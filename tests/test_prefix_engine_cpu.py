@@ -129,6 +129,12 @@ def test_prefixes_with_adapters(tiny_dirs, emu):
     rids = [eng.add_request(tail, _greedy(5), prefix=p, adapter="a"), eng.add_request(tail, _greedy(5), prefix=q), eng.add_request(tail, _greedy(5), prefix=p, adapter="a")]
     while eng.has_unfinished():
         eng.step()
+    assert eng.generate([tail, tail[:2]], _greedy(4), adapters="a", prefix=p) == \
+        [plain.greedy_generate(cfg, adapter_cases.merged(W, pairs, 1.0), tokens + t, 4) for t in (tail, tail[:2])]
+    for wrong in (dict(prefix=p), dict(prefix=q, adapters=[None, "a"]), dict(prefix=77)):
+        with pytest.raises(ValueError):
+            eng.generate([tail, tail], _greedy(2), **wrong)
+    assert not eng.has_unfinished()
     with_one = plain.greedy_generate(cfg, adapter_cases.merged(W, pairs, 1.0), tokens + tail, 5)
     assert [eng.request(r).output for r in rids] == [with_one, plain.greedy_generate(cfg, W, tokens + tail, 5), with_one]
     eng.release_prefix(p)
