@@ -257,3 +257,11 @@ def test_a_captured_step_keeps_the_runs_that_save_most(tiny_dirs, emu):
     assert kept == [(2, 16 * (g + 1) if g >= 2 else 0) for g in range(10)]
     assert runner._shared_bounds(rids) == (256, 256, 8)      # (keys for themselves: 17 to 33)
     assert runner._shared_bounds(rids[:6]) == (256, 256, 4) and runner._shared_bounds(rids[:2]) == (256, 256, 1)
+
+
+def test_when_shared_keys_pay():
+    """By what reading them once saves a layer: less for short portions, more for long ones."""
+    from tempura_amd.kernels import ops
+    mib = 1 << 20
+    for longest, least in ((1, 96), (2, 8), (64, 8), (65, 96), (128, 96), (512, 384), (2048, 1536)):
+        assert ops.shared_keys_pay(least * mib, longest) and not ops.shared_keys_pay(least * mib - 1, longest)
