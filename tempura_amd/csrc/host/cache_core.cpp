@@ -77,7 +77,6 @@ struct Pool {
 struct Request {
   bool live = false;
   int num_tokens = 0;                      // tokens whose keys and values are in the cache
-  int shared_tokens = 0;                   // of them, those in pages that another request wrote (whole pages)
   std::vector<std::vector<int>> tables;    // per group: logical page -> physical page, -1 = none
   std::vector<int> first_live;             // per group: first logical page still held
 };
@@ -109,6 +108,7 @@ struct Core {
   std::vector<Pool> pools;
   std::vector<Request> reqs;
   std::vector<int> free_state;
+  bool ever_shared = false;        // a request has begun with another's pages
 
   int n_groups() const { return (int)pools.size(); }
   // first logical page a query at position `start` can still see
@@ -206,7 +206,7 @@ int cc_add(void* h) {
   c->free_state.pop_back();
   Request& r = c->reqs[s];
   r.live = true;
-  r.num_tokens = r.shared_tokens = 0;
+  r.num_tokens = 0;
   r.tables.assign(c->n_groups(), {});
   r.first_live.assign(c->n_groups(), 0);
   return s;
@@ -233,7 +233,8 @@ int cc_share(void* h, int req, int donor, int num_tokens) {
       r->tables[g].push_back(p);
       ++c->pools[g].held[p];
     }
-  r->num_tokens = r->shared_tokens = num_tokens;
+  r->num_tokens = num_tokens;
+  c->ever_shared = true;
   return 0;
 }
 
@@ -327,7 +328,6 @@ int cc_truncate(void* h, int req, int num_tokens) {
       if (lp < (int)r->tables[g].size() && r->tables[g][lp] >= 0 && c->pools[g].held[r->tables[g][lp]] > 1)
         return fail("group %d: the page of position %d is shared with another request", g, num_tokens);
     }
-  r->shared_tokens = std::min(r->shared_tokens, num_tokens);
   const int keep = (num_tokens + c->page_size - 1) / c->page_size;
   for (int g = 0; g < c->n_groups(); ++g) {
     std::vector<int>& table = r->tables[g];
@@ -377,13 +377,21 @@ int cc_num_live(void* h) {
 // Share of held token places that hold no token (/root/reference/engine/src/kv_cache.rs:1066-1074).
 double cc_waste_ratio(void* h) {
   Core* c = (Core*)h;
-  long held = 0, used = 0;
+  long held = 0;
+  double used = 0;
   for (const Pool& p : c->pools) held += (long)(p.num_pages - p.num_free()) * c->page_size;
   if (held == 0) return 0.0;
-  for (const Request& r : c->reqs)
-    if (r.live)
-      for (int g = 0; g < c->n_groups(); ++g) used += std::max(0, r.num_tokens - r.shared_tokens - r.first_live[g] * c->page_size);
-  return std::max(0.0, 1.0 - (double)used / (double)held);
+  for (const Request& r : c->reqs) {
+    if (!r.live) continue;
+    for (int g = 0; g < c->n_groups(); ++g) {
+      used += std::max(0, r.num_tokens - r.first_live[g] * c->page_size);
+      if (!c->ever_shared) continue;
+      // (a page in several tables, which is full, counts once)
+      for (int p : r.tables[g])
+        if (p >= 0 && c->pools[g].held[p] > 1) used -= c->page_size * (1.0 - 1.0 / c->pools[g].held[p]);
+    }
+  }
+  return std::max(0.0, 1.0 - used / (double)held);
 }
 
 // No page lost, held twice or free while in a table; state slots likewise.

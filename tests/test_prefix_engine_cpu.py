@@ -196,10 +196,12 @@ def test_the_cache_shares_whole_pages():
         c.truncate("b", 6)
     with pytest.raises(ValueError):
         c.truncate("a", 3)
+    assert c.waste_ratio() == pytest.approx(1 - (4 + 4 + 3 + 4 + 1) / 20)      # (a's, of which the first two pages are b's too and the first is c's; b's own)
     c.truncate("a", 8)
     c.truncate("b", 4)
     assert c.shared("b") is None and c._lib.cc_check(c._h) == 0
     c.release("a")
+    assert c.waste_ratio() == 0.0      # (one page, full, that b and c have)
     assert c.free_pages() == [9] and c._lib.cc_check(c._h) == 0
     c.release("c")
     c.release("b")
