@@ -60,7 +60,7 @@ struct PrefixArgs {
   int shared_steps, own_steps;   // steps of 32 keys a part has
   int shared_parts, parts;   // a row's places for parts: those of the shared keys, all
   float scale_log2;          // scale * log2(e)
-  float cap_log2, cap_in;    // scores under a cap: cap * log2(e), and what turns q . k into 2 log2(e) score / cap; 0: no cap
+  float cap_log2, cap_in;    // scores under a cap: cap * log2(e), and what turns q . k into score / cap (bfloat16: 2 log2(e) score / cap); 0: no cap
 };
 
 __device__ inline unsigned pa_pack(float a, float b) {
@@ -169,17 +169,20 @@ __device__ inline void prefix_scores(const pa_u32x4 (&kk)[2][KF], const pa_u32x4
       }
 }
 
-// Scores under a cap: cap * tanh(x) with tanh(x) = 1 - 2 / (2^(2 x log2 e) + 1), in units of log 2; both limits come out right (2^large is
-// infinite, its reciprocal 0).
-template <int NQ>
+// Scores under a cap, cap * tanh(score / cap), in units of log 2.  float32: tanhf, exact to a few half steps of the result.  bfloat16: tanh(x) = 1 - 2 / (2^(2 x log2 e) + 1);
+// both limits come out right (2^large is infinite, its reciprocal 0), but it is a difference of numbers near the cap, off by a few 1e-8 of the cap (1e-5 of a score
+// at a cap of 100, where rounding the weights to bfloat16 is 4e-3 of each), which for float32 would grow beyond everything else.
+template <int E, int NQ>
 __device__ inline void prefix_cap(const PrefixArgs& a, pa_f32x4 (&s)[NQ][2]) {
 #pragma unroll
   for (int nq = 0; nq < NQ; ++nq)
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        s[nq][t][r] = fmaf(-2.0f * a.cap_log2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[nq][t][r] * a.cap_in) + 1.0f), a.cap_log2);
+      for (int r = 0; r < 4; ++r) {
+        const float x = s[nq][t][r] * a.cap_in;
+        s[nq][t][r] = E == 4 ? a.cap_log2 * tanhf(x) : fmaf(-2.0f * a.cap_log2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.0f), a.cap_log2);
+      }
 }
 
 // Keys outside the part or above the row's limit are not in the sums.
@@ -379,7 +382,7 @@ __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, c
       pa_f32x4 sc[NQ][2];
       pa_u32x4 pf[NQ][VF];
       prefix_scores<E, NQ, KF>(kk, qf, sc);
-      if (cap > 0.f) prefix_cap<NQ>(a, sc);
+      if (cap > 0.f) prefix_cap<E, NQ>(a, sc);
       if (j0 < w.first || j0 + 32 > w.end || w.limit0 < j0 + 31) prefix_mask<E, NQ>(w, j0, g, limit, sc);
       prefix_softmax<E, NQ, DT>(scale, sc, m, l, pf, o);
       if (more) PA_WAIT_VM(KI);
@@ -527,7 +530,7 @@ __device__ inline void prefix_part_rows(const PrefixArgs& a, unsigned char* stag
     pa_u32x4 pf[NQ][VF];
     prefix_scores<E, NQ, KF>(kk, qf, sc);
     at.read_values(base, vv);
-    if (cap > 0.f) prefix_cap<NQ>(a, sc);
+    if (cap > 0.f) prefix_cap<E, NQ>(a, sc);
     if (j0 < w.first || j0 + 32 > w.end || w.limit0 < j0 + 31) prefix_mask<E, NQ>(w, j0, g, limit, sc);
     prefix_softmax<E, NQ, DT>(scale, sc, m, l, pf, o);
     L::arrived(vv);
@@ -794,7 +797,7 @@ extern "C" int tp_prefix_attention(const void* q, const void* k_cache, const voi
   a.own_steps = own_steps;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.cap_log2 = softcap * 1.4426950408889634f;
-  a.cap_in = softcap > 0.f ? 2.0f * a.scale_log2 / softcap : 0.f;
+  a.cap_in = softcap > 0.f ? (dt == TP_BF16 ? 2.0f * a.scale_log2 : scale) / softcap : 0.f;
   const long of_shared = (long)shared_blocks * shared_parts, blocks = (of_shared + (long)a.own_rows * requests * own_parts) * kv_heads;
   TP_REQUIRE(blocks < (1L << 31), "prefix_attention: too many blocks");
   a.shared_blocks = (int)of_shared;

@@ -79,6 +79,14 @@ def test_joins(monkeypatch, dtype, heads, dim, parts):
 
 
 @pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("cap", [50.0, 1000.0, 30000.0])
+def test_caps_far_above_the_scores(monkeypatch, form, cap):
+    """float32 scores small beside their cap are as exact as scores without one: cap * tanh(score / cap) is a product of a few roundings, each relative to the score."""
+    s = P.step([(5, 560), (1, 0)], [3, 40, 64, 100, 1, 7], [1, 1, 2, 1, 1, 1], 8, 2, 64, 16, F32, seed=int(cap))
+    check(monkeypatch, s, form, 4, 2, cap=cap)
+
+
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_the_same_call_gives_the_same_bits(monkeypatch, form, dtype):
     s = P.step([(9, 640)], [1 + (61 * i) % 200 for i in range(9)], [1, 4, 1, 9, 1, 1, 30, 1, 2], 8, 2, 128, 16, dtype, seed=2)
