@@ -262,25 +262,90 @@ __device__ inline void prefix_clear(int end, int j0, int g, pa_u32x4 (&vv)[DT][V
   }
 }
 
+// acc += a . b over a step's keys, of one tile of elements and one of rows
+template <int E, int VF>
+__device__ inline void prefix_product(const pa_u32x4 (&a)[VF], const pa_u32x4 (&b)[VF], pa_f32x4& acc) {
+  if constexpr (E == 2) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, a[0]), __builtin_bit_cast(pa_bf16x8, b[0]), acc, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const pa_f32x4 x = __builtin_bit_cast(pa_f32x4, a[t]), y = __builtin_bit_cast(pa_f32x4, b[t]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], acc, 0, 0, 0);
+    }
+  }
+}
+
 // o += values x probabilities
 template <int E, int NQ, int DT, int VF>
 __device__ inline void prefix_values(const pa_u32x4 (&vv)[DT][VF], const pa_u32x4 (&pf)[NQ][VF], pa_f32x4 (&o)[NQ][DT]) {
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
+    for (int nq = 0; nq < NQ; ++nq) prefix_product<E, VF>(vv[dt], pf[nq], o[nq][dt]);
+}
+
+// Where a row may not see all of the step's keys a value that is not finite has to stay away from the rows in front of it (0 * Inf and 0 * NaN are not 0).  If there is
+// one, which portions of numbers never have, zeros take the place of such values, and the sums get what they would have brought: a product counts for each row and
+// element those that the row sees, 1 for a positive infinity, 64 for a negative one and 4,096 for what is no number (at most 32 of each: exact).  (In integer
+// arithmetic: comparisons' masks would take the scalar registers that the steps' addresses live in.)
+template <int E, int NQ, int DT, int VF>
+__device__ inline void prefix_odd_values(const PartRows& w, int j0, int g, const int (&limit)[NQ], pa_u32x4 (&vv)[DT][VF], pa_f32x4 (&o)[NQ][DT]) {
+  constexpr unsigned EXP = E == 2 ? 0x7f807f80u : 0x7f800000u, STEP = E == 2 ? 0x00800080u : 0x00800000u, TOP = E == 2 ? 0x80008000u : 0x80000000u;
+  unsigned odd = 0;      // (an exponent of all ones carries into the sign's place)
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+    for (int t = 0; t < VF; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) odd |= ((vv[dt][t][e] & EXP) + STEP) & TOP;
+  if (__builtin_amdgcn_ballot_w64(odd != 0) == 0) return;
+  auto all = [](unsigned n) { return 0u - min(n, 1u); };      // all bits, unless n is 0
+  constexpr unsigned ONE = 0x3f80u, MINUS = 0x4280u, NONE = 0x4580u;      // 1, 64 and 4,096: the upper halves of their float32 bits
+  pa_u32x4 sees[NQ][VF];
+#pragma unroll
+  for (int nq = 0; nq < NQ; ++nq) {
+    __builtin_amdgcn_sched_barrier(0);
+    const int from = max(w.first, j0), upto = max(from, min(w.end - 1, limit[nq]) + 1);
+    auto seen = [&](int key) { return (unsigned)((from - 1 - key) >> 31) & (unsigned)((key - upto) >> 31) & ONE; };
+#pragma unroll
+    for (int t = 0; t < VF; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = j0 + (E == 2 ? 8 * g + 2 * e : 16 * t + 4 * g + e);
+        sees[nq][t][e] = E == 2 ? seen(key) | seen(key + 1) << 16 : seen(key) << 16;
+      }
+  }
+  // (the upper 16 bits of a float32 value say whether it is finite, and its sign; the lower ones beside them whether it is an infinity)
+  auto mark = [&](unsigned v, unsigned rest) {
+    const unsigned none = all((v & 0x7fu) | rest), minus = all(v & 0x8000u);
+    return all(((v & 0x7f80u) + 0x80u) & 0x8000u) & ((none & NONE) | (~none & ((minus & MINUS) | (~minus & ONE))));
+  };
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    pa_u32x4 marks[VF];
+#pragma unroll
+    for (int t = 0; t < VF; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        __builtin_amdgcn_sched_barrier(0);      // (one behind the other: no registers beyond those of the steps without such values)
+        const unsigned v = vv[dt][t][e], hi = mark(v >> 16, E == 4 ? v & 0xffffu : 0u), lo = E == 2 ? mark(v & 0xffffu, 0u) : 0u;
+        marks[t][e] = hi << 16 | lo;
+        vv[dt][t][e] = v & ~(E == 2 ? (all(hi) & 0xffff0000u) | (all(lo) & 0x0000ffffu) : all(hi));
+      }
+#pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
-      if constexpr (E == 2) {
-        o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, vv[dt][0]), __builtin_bit_cast(pa_bf16x8, pf[nq][0]),
-                                                            o[nq][dt], 0, 0, 0);
-      } else {
+      pa_f32x4 count = {0.f, 0.f, 0.f, 0.f};
+      prefix_product<E, VF>(marks, sees[nq], count);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const pa_f32x4 vv4 = __builtin_bit_cast(pa_f32x4, vv[dt][t]), p4 = __builtin_bit_cast(pa_f32x4, pf[nq][t]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[nq][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(vv4[e], p4[e], o[nq][dt], 0, 0, 0);
-        }
+      for (int r = 0; r < 4; ++r) {
+        const unsigned n = (unsigned)count[r];
+        const float plus = __builtin_bit_cast(float, all(n & 63u) & 0x7f800000u), minus = __builtin_bit_cast(float, all(n & 4032u) & 0xff800000u);
+        o[nq][dt][r] += (plus + minus) + __builtin_bit_cast(float, all(n >> 12) & 0x7fc00000u);
       }
     }
+  }
 }
 
 // q of a wave's rows from `at` of the part's on, their places among all (token, head) rows and the last key each sees.
@@ -300,9 +365,9 @@ __device__ inline void prefix_queries(const PrefixArgs& a, const PartRows& w, in
 }
 
 // Few rows: every wave takes all of them and a run of the part's steps, through a ring of its own of one step, filled again as soon as its
-// fragments are in registers; no barrier until the waves' sums are added.  (Two blocks a CU: eight steps on their way.)  NT: keys and values are read
-// by one block only.
-template <int E, int D, int NQ, bool NT>
+// fragments are in registers; no barrier until the waves' sums are added.  (Two blocks a CU: eight steps on their way.)  OWN: a request's own keys,
+// which one block reads and of which a row may not see all.
+template <int E, int D, int NQ, bool OWN>
 __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, const PartRows& w, int kvh) {
   using L = PrefixLane<E, D>;
   constexpr int KF = L::KF, DT = L::DT, VF = L::VF, KI = L::KI;
@@ -337,14 +402,14 @@ __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, c
     const unsigned char* b0 = kbase + (size_t)(unsigned)pp0 * page_bytes + (unsigned)((j0 & pmask) * (D * E));
     const unsigned char* b1 = kbase + (size_t)(unsigned)pp1 * page_bytes + (unsigned)((j1 & pmask) * (D * E));
 #pragma unroll
-    for (int t = 0; t < KI; ++t) prefix_copy<NT>(t >= KI / 2 ? b1 : b0, koff[t], ring + t * 1024);
+    for (int t = 0; t < KI; ++t) prefix_copy<OWN>(t >= KI / 2 ? b1 : b0, koff[t], ring + t * 1024);
   };
   auto issue_values = [&](int i) __attribute__((always_inline)) {
     const int j0 = base16 + (w0 + i) * 32, j1 = min(j0 + 16, last16);
     const unsigned char* b0 = vbase + (size_t)(unsigned)pp0 * page_bytes + (unsigned)((j0 & pmask) * E);
     const unsigned char* b1 = vbase + (size_t)(unsigned)pp1 * page_bytes + (unsigned)((j1 & pmask) * E);
 #pragma unroll
-    for (int t = 0; t < KI; ++t) prefix_copy<NT>(((t & 1) ? b1 : b0) + (size_t)((t >> 1) * L::VD * E) * ps, voff, ring + (KI + t) * 1024);
+    for (int t = 0; t < KI; ++t) prefix_copy<OWN>(((t & 1) ? b1 : b0) + (size_t)((t >> 1) * L::VD * E) * ps, voff, ring + (KI + t) * 1024);
   };
   pa_u32x4 qf[NQ][KF];
   int limit[NQ];
@@ -394,6 +459,7 @@ __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, c
         if (i + 2 < n) pages_of(i + 2);
       }
       if (j0 + 32 > w.end) prefix_clear<E, DT, VF>(w.end, j0, g, vv);
+      if (OWN && w.limit0 < j0 + 31) prefix_odd_values<E, NQ, DT, VF>(w, j0, g, limit, vv, o);
       prefix_values<E, NQ, DT, VF>(vv, pf, o);
     }
   }
@@ -441,7 +507,7 @@ __device__ inline void prefix_part(const PrefixArgs& a, unsigned char* stages, c
 
 // Many rows: the four waves take 16 * NQ rows each and walk the part's steps together, through a ring of NS steps that all of them fill, a quarter each,
 // NS - 1 steps ahead; one barrier a step.  So a CU loads a step once for 64 * NQ rows, and one wave's products run beside another's exponentials.
-template <int E, int D, int NQ, int NS>
+template <int E, int D, int NQ, int NS, bool OWN>
 __device__ inline void prefix_part_rows(const PrefixArgs& a, unsigned char* stages, const PartRows& w, int kvh) {
   using L = PrefixLane<E, D>;
   constexpr int KF = L::KF, DT = L::DT, VF = L::VF, KI = L::KI;
@@ -535,6 +601,7 @@ __device__ inline void prefix_part_rows(const PrefixArgs& a, unsigned char* stag
     prefix_softmax<E, NQ, DT>(scale, sc, m, l, pf, o);
     L::arrived(vv);
     if (j0 + 32 > w.end) prefix_clear<E, DT, VF>(w.end, j0, g, vv);
+    if (OWN && w.limit0 < j0 + 31) prefix_odd_values<E, NQ, DT, VF>(w, j0, g, limit, vv, o);
     prefix_values<E, NQ, DT, VF>(vv, pf, o);
   }
   PA_WAIT_VM(0);       // (nothing is on its way into LDS when the block ends)
@@ -552,10 +619,10 @@ __device__ inline void prefix_part_rows(const PrefixArgs& a, unsigned char* stag
 }
 
 // NS 0: 16 * NQ rows whose keys the waves share out; else 64 * NQ rows, 16 * NQ for a wave.
-template <int E, int D, int NQ, int NS, bool NT>
+template <int E, int D, int NQ, int NS, bool OWN>
 __device__ inline void prefix_block(const PrefixArgs& a, unsigned char* stages, const PartRows& w, int kvh) {
-  if constexpr (NS > 0) prefix_part_rows<E, D, NQ, NS>(a, stages, w, kvh);
-  else prefix_part<E, D, NQ, NT>(a, stages, w, kvh);
+  if constexpr (NS > 0) prefix_part_rows<E, D, NQ, NS, OWN>(a, stages, w, kvh);
+  else prefix_part<E, D, NQ, OWN>(a, stages, w, kvh);
 }
 
 // NQS, NSS: of blocks with shared keys, the tiles of 16 rows (of a wave, if NSS > 0) and the steps of a ring that the waves share (0: each has its own);

@@ -88,6 +88,37 @@ def test_caps_far_above_the_scores(monkeypatch, form, cap):
 
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("dim", [128, 32])
+def test_what_is_not_finite_behind_a_token(monkeypatch, form, dtype, dim):
+    """Keys and values of a request's later tokens that are infinite or no numbers leave the tokens in front of them as they are, and give those that see them what the
+    definition gives: an element whose values hold one infinity is infinite, with two of opposite signs or with what is no number it is none."""
+    new, own, inf = [1, 9, 40, 40], [20, 30, 61, 75], float("inf")
+    s = P.step([(4, 80)], own, new, 8, 2, dim, 16, dtype, seed=dim, cut=5)
+    last = dict(enumerate(s["ctx"].tolist()))
+
+    def put(request, behind, name, values):      # (into the key or value `behind` places in front of the request's last)
+        at = last[request] - 1 - behind
+        page = int(s["tables"][request, at // 16])
+        row = s[name][page, :, at % 16] if name == "k" else s[name][page, :, :, at % 16]
+        for element, x in values.items():
+            row[:, element] = x
+    put(1, 3, "v", {0: inf, 5: -inf, 17: float("nan")})
+    put(1, 0, "v", {0: -inf, 5: -inf})
+    put(2, 20, "v", {3: inf, 31: inf})
+    put(2, 11, "v", {3: inf, 4: -inf, dim - 1: float("nan")})
+    put(3, 0, "v", {i: inf for i in range(dim)})
+    put(3, 18, "k", {2: float("nan")})
+    want, size, reach = P.exact(s)
+    got = run(monkeypatch, s, form, 2, 1)
+    finite = torch.isfinite(want)
+    assert bool((~finite).any()) and bool(finite[: 1 + 5].all())
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[want.abs() == inf], want[want.abs() == inf])
+    tol = P.tolerance(s, want, torch.where(finite, size, torch.zeros_like(size)), torch.where(torch.isfinite(reach), reach, torch.zeros_like(reach)))
+    assert float(((got - want).abs() - tol)[finite].max()) <= 0
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_the_same_call_gives_the_same_bits(monkeypatch, form, dtype):
     s = P.step([(9, 640)], [1 + (61 * i) % 200 for i in range(9)], [1, 4, 1, 9, 1, 1, 30, 1, 2], 8, 2, 128, 16, dtype, seed=2)
     first = run(monkeypatch, s, form, 3, 2)
