@@ -1,7 +1,49 @@
 """When shared keys are read once for all, and how such a launch is laid out, on the host."""
 import random
 
+import pytest
 import torch
+
+
+@pytest.fixture
+def launched(monkeypatch):
+    """What the entry point hands to the library: its name for steps that read shared keys once, "paged" for the others."""
+    from tempura_amd.kernels import ops
+    made = []
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)      # (what host tensors name as theirs)
+    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_call", lambda name, *args, tag=None: made.append((name, args)))
+    monkeypatch.setattr(ops, "paged_attention", lambda *a, **kw: made.append(("paged", kw)))
+    return made
+
+
+def attend(launched, singles, portion, shared, own, portion_own, heads=32, kv=8, dim=128, dtype=torch.bfloat16, page=16, **kw):
+    """The kind of launch of a step of one portion and single tokens behind the same keys."""
+    from tempura_amd.kernels import ops
+    new = ([portion] if portion else []) + [1] * singles
+    ctx = ([shared + portion_own] if portion else []) + [shared + own] * singles
+    r, n, longest = len(new), sum(new), max(ctx)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    del launched[:]
+    ops.prefix_attention(torch.empty(n, heads, dim, dtype=dtype), torch.empty(2, kv, page, dim, dtype=dtype), torch.empty(2, kv, dim, page, dtype=dtype),
+                         torch.zeros(r, -(-longest // page), dtype=torch.int32), torch.tensor([0] + new).cumsum(0).int(), i32(ctx),
+                         i32([i for i, t in enumerate(new) for _ in range(t)]), 0.1, ops.SharedKeys([r], [shared], "cpu"), max(new), longest,
+                         max_own_len=max(own, portion_own if portion else 0), num_single=singles, **kw)
+    return "paged" if launched[0][0] == "paged" else "once"
+
+
+def test_portions_beside_requests_with_many_keys_of_their_own(launched):
+    """A part of own keys is walked by one block: not beside a portion, where that would take longer than reading the shared keys for each request."""
+    go = lambda *a, **kw: attend(launched, *a, **kw)  # noqa: E731
+    assert go(32, 512, 8192, 32768, 512) == "paged" and go(32, 512, 8192, 8192, 512) == "paged" and go(32, 128, 2048, 4000, 128) == "paged"
+    assert go(8, 128, 2048, 100, 20000) == "paged"
+    assert go(32, 512, 8192, 1000, 512) == "once" and go(8, 128, 2048, 1000, 128) == "once" and go(32, 64, 2048, 1000, 64) == "once"
+    assert go(32, 2, 2048, 16000, 2) == "once"         # (blocks of 16 rows are cut over their waves and parts)
+    assert go(33, 0, 8192, 32768, 0) == "once"         # (and single tokens alone)
+    for dtype in (torch.bfloat16, torch.float32):
+        for portion in (30, 100, 500):
+            kinds = [go(16, portion, 8192, own, portion, dtype=dtype) for own in (100, 1000, 4000, 16000, 64000, 256000)]
+            assert kinds == sorted(kinds, key=lambda k: k == "paged") and kinds[0] == "once" and kinds[-1] == "paged"
 
 
 def test_blocks_hold_the_rows_of_every_step():
