@@ -209,6 +209,10 @@ class ModelRunner:
         # requests may begin with pages of another where nothing but the paged cache carries what came before
         self.can_share = self.cache.shareable and not self.pools.state
         self._key_bytes = max([g.page_bytes(1, 4 if (cache_dtype or model.dtype) == torch.float32 else 2) for g in model.cache_groups], default=0)
+        # (and attention reads what they share once where a layer of the model has sizes that the kernel is built for)
+        self._kv_dtype = cache_dtype or model.dtype
+        self._reads_once = any(part.reads_shared_keys() and ops.prefix_attention_ok(self._kv_dtype, part.key_dim, part.value_dim, self.page_size)
+                               for layer in model.layers for part in layer.parts() if hasattr(part, "reads_shared_keys"))
         self._shared_keys: Dict[tuple, ops.SharedKeys] = {}
         #: host time spent packing the inputs of eager steps, and how many such steps there were
         self.host_seconds = {"pack": 0.0}
@@ -372,7 +376,9 @@ class ModelRunner:
             best = set(sorted(range(len(runs)), key=lambda i: ((1 - runs[i][0]) * runs[i][1], i))[:most])
             runs = [(c, v if i in best else 0) for i, (c, v) in enumerate(runs)]
         saved = sum((c - 1) * v for c, v in runs)
-        return runs if saved > 0 and ops.shared_keys_pay(saved * self._key_bytes, longest) else None
+        if saved <= 0 or ops.shared_keys_pay_bytes == 0:
+            return runs if saved > 0 else None
+        return runs if self._reads_once and ops.prefix_keys_pay(runs, self._kv_dtype, longest) and ops.shared_keys_pay(saved * self._key_bytes, longest) else None
 
     def _adapted(self, rids) -> bool:
         return bool(self.adapter_of) and any(rid in self.adapter_of for rid in rids)

@@ -1510,7 +1510,7 @@ def attention_rows(rows, col0: int, ctx, group: int, heads: int, kvh: int, dim: 
 
 
 #: the engine's steps of single tokens, and of portions of up to 128, read shared keys once for all where that saves at least so many bytes of keys and
-#: values a layer; of longer portions as many times more as they are longer, of portions up to 64 a twelfth.  (Single tokens behind shared keys, 32 heads of
+#: values a layer (0: they leave it to ``prefix_attention``); of longer portions as many times more as they are longer, of portions up to 64 a twelfth.  (Single tokens behind shared keys, 32 heads of
 #: 128 over 8 key heads, bf16, a captured step of four layers with embedding and head, us, once for all / each for itself: 2 requests of 8,192 keys,
 #: 34 MB a layer saved, 545 / 542; 4 of 4,096, 50 MB, 541 / 542; 8 of 2,048, 59 MB, 550 / 553; 16 of 2,048, 126 MB, 629 / 648; 32 of 1,024, 130 MB, 685 / 678;
 #: 8 of 8,192, 235 MB, 570 / 613; 32 of 2,048, 260 MB, 692 / 703; 32 of 8,192, 1,040 MB, 732 / 865; 64 of 8,192, 2,110 MB, 784 / 1,206.  The attention alone of
@@ -1520,7 +1520,8 @@ shared_keys_pay_bytes = 96 << 20
 
 
 def shared_keys_pay(saved_bytes: int, longest: int) -> bool:
-    """Whether a step whose longest portion has ``longest`` tokens reads shared keys once for all, which saves so many bytes a layer."""
+    """Whether a step whose longest portion has ``longest`` tokens reads shared keys once for all, which saves so many bytes a layer (``prefix_keys_pay``
+    has to allow it too)."""
     least = shared_keys_pay_bytes
     return saved_bytes >= (least if longest == 1 else least // 12 if longest <= 64 else least * max(128, longest) // 128)
 
@@ -1534,6 +1535,15 @@ def shared_keys_pay(saved_bytes: int, longest: int) -> bool:
 #: 10.6 / 9.6, 12.1 / 13.9, 14.2 / 33.6; of 64 behind 256, 1,024, 4,096 27 / 16, 42 / 35, 69 / 75; of 256 behind 1,024 and 4,096 104 / 88, 216 / 261;
 #: of 512 behind 4,096 450 / 408, 4 of 512 behind 8,192 342 / 438.)
 prefix_least_keys, prefix_least_saved = (768, 512, 192), 48 << 10
+
+
+def prefix_keys_pay(runs, dtype: torch.dtype, longest: int) -> bool:
+    """Whether runs [(requests, shared keys)] share enough keys for a step whose longest portion has ``longest`` tokens to read them once for all."""
+    least = prefix_least_keys[int(dtype == torch.float32)] if longest == 1 else max(prefix_least_keys[2], min(prefix_least_keys[2], 16) * longest)
+    most = max((v for _, v in runs), default=0)
+    return most > 0 and (most >= least or (longest == 1 and sum((c - 1) * v for c, v in runs) >= prefix_least_saved))
+
+
 #: Beside a longer portion the own keys of single tokens lie in blocks of as many rows as the portion has, a whole part of them in one block step by step, where
 #: ``paged_attention`` spreads them over blocks of their own.  Shared keys are read once for all where a part of own keys has at most so many steps of 32 keys, and one
 #: more for every so many steps of shared keys.  (Once for all / each for itself, us, 32 heads of 128 over 8, bf16, portion and single tokens, own keys each: behind 2,048
@@ -1571,6 +1581,11 @@ class SharedKeys:
         self._runs, self._plans, self._bound = [(c, v) for c, v in runs if v], {}, False
         data = torch.tensor(starts + [v for _, v in runs] + [v for c, v in runs for _ in range(c)], dtype=torch.int32).to(device)
         self.starts, self.keys, self.each = data[: self.groups + 1], data[self.groups + 1: 2 * self.groups + 1], data[2 * self.groups + 1:]
+
+    def _keep(self, key: tuple, plan) -> None:
+        if len(self._plans) >= 512:
+            self._plans.clear()
+        self._plans[key] = plan
 
     @classmethod
     def captured(cls, data: torch.Tensor, requests: int, groups: int, max_keys: int) -> "SharedKeys":
@@ -1620,14 +1635,14 @@ def prefix_attention_ok(dtype: torch.dtype, dim: int, value_dim: int, page_size:
 def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor, cu_seqlens: torch.Tensor,
                      context_lens: torch.Tensor, token_req: torch.Tensor, scale: float, shared: SharedKeys, max_q_len: int, max_context_len: int,
                      max_own_len: Optional[int] = None, num_single: Optional[int] = None, sink: Optional[torch.Tensor] = None,
-                     softcap: float = 0.0) -> torch.Tensor:
+                     softcap: float = 0.0, step: Optional[dict] = None) -> torch.Tensor:
     """``paged_attention`` (without a window) of a step whose requests begin with the same keys: the same operands and result, but the pages
     that the requests of a run of ``shared`` have in common are read once for all of them.  Every request's block table names its shared pages
     as well; its new tokens lie behind its shared keys.  ``max_own_len``: the most keys that a request has behind its shared ones, its
     new tokens among them (a bound, at least the longest; None: ``max_context_len``).  Every row of q belongs to
     a request, whose index in the batch ``token_req`` gives.  Sizes that the kernel is not built for
     (``prefix_attention_ok``), steps without shared keys or with few (``prefix_least_keys``), and portions beside requests with many keys of
-    their own (``prefix_own_steps``) run ``paged_attention``."""
+    their own (``prefix_own_steps``) run ``paged_attention``, which gets ``step`` as its ``shared``."""
     if _backend is not None:
         return _backend.prefix_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, shared, max_q_len,
                                          max_context_len, max_own_len, num_single, sink, softcap)
@@ -1641,9 +1656,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     plan = shared._plans.get(key)
     if plan is None:
         plan = _prefix_checked(q, k_cache, v_cache, block_tables, shared, int(max_q_len), (own + 255) // 256 * 256)
-        if len(shared._plans) >= 256:
-            shared._plans.clear()
-        shared._plans[key] = plan
+        shared._keep(key, plan)
     n, r, heads, sizes, room = plan
     if not shared.max_keys < max(1, max_context_len) <= block_tables.shape[1] * k_cache.shape[2]:
         raise KernelError("prefix_attention: the longest context must be longer than the shared keys (new tokens lie behind them) and fit the block table")
@@ -1654,7 +1667,7 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
         _need(sink.dtype == torch.float32 and sink.numel() == heads, "prefix_attention: sink must be float32 [heads]")
     if sizes is None:
         return paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, 0, max_q_len, max_context_len,
-                               num_single, sink=sink, softcap=softcap)
+                               num_single, sink=sink, softcap=softcap, shared=step)
     out = q.new_empty((n, heads * q.shape[2]))
     if n == 0:
         return out
@@ -1679,21 +1692,33 @@ def _prefix_checked(q, k_cache, v_cache, block_tables, shared: SharedKeys, max_q
     if shared.requests != r:
         raise KernelError(f"prefix_attention: runs of {shared.requests} requests for a batch of {r}")
     _need(n >= r and max_q_len >= 1, "prefix_attention: every request brings at least one token")
-    if shared.max_keys == 0 or not prefix_attention_ok(q.dtype, d, vd, page_size):
+    layout = _prefix_layout(shared, n, heads, kvh, d, vd, page_size, q.dtype, max_q_len, own)
+    if layout is None:
         return n, r, heads, None, 0
-    least = prefix_least_keys[int(q.dtype == torch.float32)] if max_q_len == 1 else max(prefix_least_keys[2], min(prefix_least_keys[2], 16) * max_q_len)
-    many = max_q_len == 1 and sum((c - 1) * v for c, v in shared._runs) >= prefix_least_saved
-    if shared.max_keys < least and not many and not shared._bound:
-        return n, r, heads, None, 0
-    rows_shared, rows_own, blocks, shared_steps, shared_parts, own_steps, own_parts = _prefix_plan(shared, r, n, heads // kvh, kvh, max_q_len, own, d, q.dtype)
-    if rows_own > 16 and own_steps > prefix_own_steps + -(-shared.max_keys // 32) // prefix_own_share:
-        return n, r, heads, None, 0
-    sizes = (_dt(q), width, n, r, shared.groups, heads, kvh, d, page_size, max_q_len, rows_shared, rows_own, blocks, shared_steps, shared_parts,
-             own_steps, own_parts)
-    room = n * heads * (shared_parts + own_parts) * (d + 2) + 2
-    if room * 4 > prefix_scratch_limit:
-        return n, r, heads, None, 0
-    return n, r, heads, (ctypes.c_int * len(sizes))(*sizes), room
+    sizes = (_dt(q), width, n, r, shared.groups, heads, kvh, d, page_size, max_q_len) + layout
+    return n, r, heads, (ctypes.c_int * len(sizes))(*sizes), n * heads * (layout[4] + layout[6]) * (d + 2) + 2
+
+
+def _prefix_layout(shared: SharedKeys, n: int, heads: int, kvh: int, dim: int, value_dim: int, page_size: int, dtype: torch.dtype, max_q_len: int, own: int):
+    """``_prefix_plan`` of a step that reads shared keys once for all, None of one that runs ``paged_attention``."""
+    key = (n, heads, kvh, dim, value_dim, page_size, dtype, max_q_len, own)
+    if key in shared._plans:
+        return shared._plans[key]
+    plan = None
+    if shared.max_keys and prefix_attention_ok(dtype, dim, value_dim, page_size) and (shared._bound or prefix_keys_pay(shared._runs, dtype, max_q_len)):
+        plan = _prefix_plan(shared, shared.requests, n, heads // kvh, kvh, max_q_len, own, dim, dtype)
+        _, rows_own, _, _, shared_parts, own_steps, own_parts = plan
+        if (rows_own > 16 and own_steps > prefix_own_steps + -(-shared.max_keys // 32) // prefix_own_share) \
+                or (n * heads * (shared_parts + own_parts) * (dim + 2) + 2) * 4 > prefix_scratch_limit:
+            plan = None
+    shared._keep(key, plan)
+    return plan
+
+
+def prefix_reads_once(shared: SharedKeys, tokens: int, heads: int, k_cache: torch.Tensor, v_cache: torch.Tensor, max_q_len: int, max_own_len: int) -> bool:
+    """Whether ``prefix_attention`` of such a step reads shared keys once for all (else it is ``paged_attention``, and so is what a program does without it)."""
+    _, kvh, page_size, dim = k_cache.shape
+    return _prefix_layout(shared, tokens, heads, kvh, dim, v_cache.shape[2], page_size, k_cache.dtype, int(max_q_len), (max_own_len + 255) // 256 * 256) is not None
 
 
 #: What a launch of ``prefix_attention`` takes (us), by element type: a block's beginning, seen by itself and among others; a block with own keys and a step

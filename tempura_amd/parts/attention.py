@@ -267,6 +267,10 @@ class PagedAttention(TakesAdapters, Mixer):
         w = self.spec.weights
         return self._paired(b) if name in (w["q"], w["k"]) else b
 
+    def reads_shared_keys(self) -> bool:
+        """Whether keys that requests of a step share may be read once for all here (``ops.prefix_attention``)."""
+        return self.window is None and not self.chunk and self.distance_bias is None and not self.gate and self.scale > 0
+
     def cache_spec(self):
         kind, span = ("window", self.window) if self.window is not None else ("chunk", self.chunk) if self.chunk else ("full", None)
         if self.keep_first:
@@ -303,10 +307,11 @@ class PagedAttention(TakesAdapters, Mixer):
         step = {**into, "shared": shared}
         a, attended = None, False
         # (requests that begin with the same pages: keys that all of them see are read once)
-        shared_keys = getattr(ctx, "shared_keys", None) if self.window is None and not self.chunk and self.dist_table is None and not self.gate else None
+        shared_keys = getattr(ctx, "shared_keys", None) if self.reads_shared_keys() else None
+        once = shared_keys is not None and ops.prefix_reads_once(shared_keys, ctx.num_tokens, self.num_heads, cache.k, cache.v, ctx.max_q_len, ctx.max_own_len)
         if q is None:
             rows = self._project(x, cache, rot) if ids is None else self._project_adapted(x, ids, ctx, cache)
-            if shared_keys is None and cache.writes and (rot is not None or type(self.position).__name__ == "NoPosition") and not self.softcap and self.dist_table is None \
+            if not once and cache.writes and (rot is not None or type(self.position).__name__ == "NoPosition") and not self.softcap and self.dist_table is None \
                     and ops.attention_rows_ok(rows, ctx, self.num_heads, self.num_kv_heads, self.head_dim, self.value_dim, cache.k) \
                     and ops.attention_rows_pays(ctx, self.num_kv_heads, self.head_dim, int(self.window or 0), self.keep_first, self.chunk):
                 # single tokens: the attention takes the projection's rows itself
@@ -324,7 +329,7 @@ class PagedAttention(TakesAdapters, Mixer):
         elif shared_keys is not None:
             a = ops.prefix_attention(
                 q, cache.k, cache.v, ctx.block_tables[cache.group], ctx.cu_seqlens, ctx.context_lens, ctx.token_req, self.scale, shared_keys,
-                ctx.max_q_len, ctx.max_context_len, ctx.max_own_len, ctx.num_single, sink=self.sink_w, softcap=self.softcap)
+                ctx.max_q_len, ctx.max_context_len, ctx.max_own_len, ctx.num_single, sink=self.sink_w, softcap=self.softcap, step=shared)
         elif self.extended or self.chunk or self.softcap:
             a = ops.paged_attention(
                 q, cache.k, cache.v, ctx.block_tables[cache.group], ctx.cu_seqlens, ctx.context_lens,

@@ -83,3 +83,26 @@ def test_blocks_hold_the_rows_of_every_replay():
         ops.SharedKeys.pack(runs, r, groups, out)
         assert plan[2] >= sum(-(-(int(shared.starts[g + 1]) - int(shared.starts[g])) * group // plan[0]) for g in range(groups) if int(shared.keys[g]))
         assert plan[3] * plan[4] * 32 >= shared.max_keys
+
+
+def test_the_engine_and_the_operator_ask_the_same(launched, tiny_dirs):
+    """Keys that the operator would read for each request are no shared keys of a step, however many bytes that would save; nor are those of a model whose heads or
+    pages the kernel is not built for."""
+    from tempura_amd.kernels import ops
+    from tempura_amd.engine import Engine
+    for requests, keys, once in ((98, 256, False), (40, 640, False), (50, 512, False), (64, 768, True), (193, 256, True), (2, 800, True)):
+        assert ops.prefix_keys_pay([(requests, keys)], torch.bfloat16, 1) == once
+        assert attend(launched, requests, 0, keys, 100, 0) == ("once" if once else "paged")
+    for name, page, sizes in (("D", 16, True), ("D", 8, False), ("A", 16, False), ("E", 16, False)):
+        runner = Engine(tiny_dirs.path(name, "float32"), dtype="float32", device="cpu", page_size=page, kv_pages=256, max_batch_size=8, max_prefixes=1).runner
+        runner._key_bytes = 1 << 30
+        cache = runner.cache
+        cache.add("d"), cache.reserve("d", 640), cache.commit("d", 640)
+        for keys in (512, 496, 640):
+            for i in range(3):
+                cache.add((keys, i)), cache.share((keys, i), "d", keys)
+        assert runner._reads_once == sizes
+        for keys, enough in ((512, True), (496, False), (640, True)):       # (float32: from 512 on)
+            rids = [(keys, i) for i in range(3)]
+            assert runner._shared_runs(rids) == ([(3, keys)] if sizes and enough else None)
+            assert (runner._shared_bounds(rids) is not None) == (sizes and enough)

@@ -37,3 +37,44 @@ def test_steps_that_read_shared_keys_once(tiny_dirs, monkeypatch, launches, kw):
     assert got == [plain.greedy_generate(cfg, W, prefix + t, 9) for t in tails]
     # (two layers; eager: every step that several requests share)
     assert launches.count("tp_prefix_attention") >= (2 * 9 if kw.get("use_graph") is False else 2 * 2)
+
+
+@pytest.mark.parametrize("kind", ["rows", "plain"])
+def test_steps_that_do_not_are_as_without(launches, kind):
+    """Where each request reads its keys for itself, because they are few, a step keeps the kernels that it has without runs of requests: the one that takes the
+    projection's rows (of an attention with a norm per head), or the attention with the order of its requests; the same bits."""
+    from tempura_amd.cache import LayerCache
+    from tempura_amd.config.spec import PartSpec
+    from tempura_amd.kernels import ops
+    from tempura_amd.parts import build_part
+    heads, kv, dim, width, page, dev = 8, 2, 64, 128, 16, "cuda:0"
+    g = torch.Generator().manual_seed(1)
+    shapes = {"q": (heads * dim, width), "k": (kv * dim, width), "v": (kv * dim, width), "o": (width, heads * dim), "qn": (dim,), "kn": (dim,)}
+    weights = {n: torch.randn(*s, generator=g) * 0.1 for n, s in shapes.items()}
+    more = {"qk_norm": {"eps": 1e-6}} if kind == "rows" else {}
+    part = build_part("mixer", PartSpec("attention", {"num_heads": heads, "num_kv_heads": kv, "head_dim": dim, "scale": 0.125, **more,
+                                                      "position": PartSpec("rope", {"head_dim": dim, "rotary_dim": dim, "theta": 1e4})},
+                                        {"q": "q", "k": "k", "v": "v", "o": "o", "q_norm": "qn", "k_norm": "kn"}), width, torch.bfloat16, dev)
+    part.load_weights(lambda n: weights[n])
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    r, lens = 5, [50, 61, 49, 80, 70]
+
+    class Ctx:
+        positions, token_req, cu_seqlens, context_lens = i32(*[n - 1 for n in lens]), i32(*range(r)), i32(*range(r + 1)), i32(*lens)
+        block_tables = [i32(*[[0, 1, 2] + [3 + 3 * i + j for j in range(3)] for i in range(r)])]
+        slot_mapping = [i32(*[(3 + 3 * i + (n - 1 - 48) // page) * page + (n - 1) % page for i, n in enumerate(lens)])]
+        max_q_len, max_context_len, num_single, num_tokens, num_requests, max_own_len = 1, 80, r, r, r, 32
+        shared_keys = None
+    pools = [torch.randn(20, kv, page, dim, generator=g).to(torch.bfloat16).to(dev), torch.randn(20, kv, dim, page, generator=g).to(torch.bfloat16).to(dev)]
+    x = torch.randn(r, width, generator=g).to(torch.bfloat16).to(dev)
+
+    def step(shared_keys):
+        del launches[:]
+        Ctx.shared_keys, Ctx.shared = shared_keys, {}
+        return part.forward(x, Ctx, LayerCache(0, {"k": pools[0].clone(), "v": pools[1].clone()}, True, page, None), torch.zeros(r, width, device=dev)), list(launches), dict(Ctx.shared)
+    residual, real = [], part.forward
+    part.forward = lambda x, ctx, cache, h: (real(x, ctx, cache, h), residual.append(h))[0]
+    _, made, kept = step(None)
+    _, again, kept_again = step(ops.SharedKeys([r], [48], dev))
+    assert made == again and ("attention_rows" in made) == (kind == "rows") and kept.keys() == kept_again.keys()
+    assert torch.equal(residual[0], residual[1]) and float(residual[0].abs().max()) > 0
