@@ -930,6 +930,7 @@ class Adapters:
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, ends=None, interleaved: bool = False):
         if _backend is None:
             _dev_ok(a, b, scales)
+        _need(a.device == b.device == scales.device, "Adapters: a, b and scales must be on one device")
         _need(a.dim() == b.dim() == 3 and a.dtype == b.dtype and a.dtype in (torch.bfloat16, torch.float32),
               "Adapters: a [slots, slices * rank, k] and b [slots, n, rank], bfloat16 or float32")
         self.slots, self.n, rank = b.shape
@@ -969,7 +970,7 @@ def adapter_linear(x: torch.Tensor, w, adapters: Adapters, ids: torch.Tensor, re
     ``max_run``: the most tokens that a request brings (0: not known)."""
     if _backend is not None:
         return _backend.adapter_linear(x, w, adapters, ids, residual)
-    _here_ok(x, ids, adapters.a, residual)
+    _here_ok(x, ids, adapters.a, residual, _w_args(w)[0])
     _need(x.dim() == 2 and x.dtype == adapters.dtype, "adapter_linear: x must be [m, k] of the adapters' type")
     m, k = x.shape
     if not (k == adapters.k and w.dim() == 2 and tuple(w.shape) == (adapters.n, k)):
