@@ -925,7 +925,8 @@ class Adapters:
     ``b`` [slots, n, rank] (both of the activations' type), ``scales`` float32 [slots].  A projection that several matrices were
     stacked into has a pair for each of its slices: ``ends`` are the columns at which they end (None: one slice), slice i has the rows
     i * rank .. of ``a``; ``interleaved``: two slices whose columns alternate by eights (``interleave_gate_up``).  Ranks that are no multiple
-    of 8 are padded with zeros here, once; otherwise the tensors are kept as they are, and what is written into them later counts."""
+    of 8 are padded with zeros here, once, and a ``b`` that is not aligned to 16 bytes is copied, both then (``a`` and ``b`` are the copies); otherwise the
+    tensors are kept as they are, and what is written into them later counts."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor, ends=None, interleaved: bool = False):
         if _backend is None:

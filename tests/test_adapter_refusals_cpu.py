@@ -41,3 +41,17 @@ def test_operands_of_several_devices(launched):
     assert not launched
     ops.adapter_linear(good["x"], good["w"], ad, good["ids"])
     assert launched == ["linear", "tp_adapter_add"]
+
+
+def test_tensors_are_kept_or_copied_as_documented(launched):
+    """Kept where the kernels can read them as they are; with ranks that are no multiple of 8, or a b at an odd place, both are copied once."""
+    from tempura_amd.kernels import ops
+    a, b, scales = torch.randn(3, 8, 64), torch.randn(3, 48, 8), torch.ones(3)
+    ad = ops.Adapters(a, b, scales)
+    assert ad.a.data_ptr() == a.data_ptr() and ad.b.data_ptr() == b.data_ptr() and ad.scales is scales
+    odd = torch.randn(3 * 48 * 8 + 1)[1:].view(3, 48, 8)
+    assert odd.data_ptr() % 16 != 0
+    ad = ops.Adapters(a, odd, scales)
+    assert ad.b.data_ptr() % 16 == 0 and torch.equal(ad.b, odd) and torch.equal(ad.a, a) and ad.a.data_ptr() != a.data_ptr()
+    ad = ops.Adapters(a[:, :5].contiguous(), b[..., :5].contiguous(), scales)
+    assert ad.rank == 8 and torch.equal(ad.a[:, :5], a[:, :5]) and torch.equal(ad.b[..., :5], b[..., :5]) and not ad.a[:, 5:].any() and not ad.b[..., 5:].any()
