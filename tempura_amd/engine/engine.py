@@ -161,7 +161,8 @@ class Engine:
         """Compute the keys and values of tokens that many requests will begin with (a system prompt, a document) and hold them; the handle
         goes to ``add_request``.  Requests share its whole pages, compute only what comes behind them, and in a step with several of them
         attention reads the shared keys once (``ops.prefix_attention``).  ``adapter``: the adapter that it is computed with, and that such
-        requests then have to name."""
+        requests then have to name.  Its pages have to be free now: no running request gives any up for it (``PagesExhausted``, and nothing is computed; steps
+        that end requests make room)."""
         tokens = [int(t) for t in token_ids]
         if len(self._prefixes) >= self.max_prefixes:
             raise ValueError(f"{len(self._prefixes)} prefixes are held, there is room for no more (max_prefixes)")
@@ -185,6 +186,7 @@ class Engine:
         if adapter is not None:
             self.runner.adapter_of[rid] = self._adapters[adapter]
         try:
+            self.runner.cache.reserve(rid, shared)
             budget = self.scheduler.config.max_num_batched_tokens
             for at in range(0, shared, budget):
                 self.runner.step([StepEntry(rid, tokens[at: min(shared, at + budget)], [])])
