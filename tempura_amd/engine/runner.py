@@ -204,6 +204,7 @@ class ModelRunner:
         self.tokens_run = 0
         self._staging = _PackedStaging(self.device)
         self._adapter_staging = _PackedStaging(self.device)
+        self._runs_staging = _PackedStaging(self.device)
         #: requests with an adapter -> its slot (whoever adds a request says so here, for as long as it runs)
         self.adapter_of: Dict[Hashable, int] = {}
         # requests may begin with pages of another where nothing but the paged cache carries what came before
@@ -349,7 +350,7 @@ class ModelRunner:
             if key not in self._shared_keys:
                 if len(self._shared_keys) >= 64:
                     self._shared_keys.clear()
-                self._shared_keys[key] = ops.SharedKeys([c for c, _ in runs], [v for _, v in runs], self.device)
+                self._shared_keys[key] = ops.SharedKeys([c for c, _ in runs], [v for _, v in runs], self.device, send=self._send_runs)
             ctx.shared_keys = self._shared_keys[key]
             each = np.repeat([v for _, v in runs], [c for c, _ in runs])
             ctx.max_own_len = int((ctx_lens - each).max())
@@ -379,6 +380,10 @@ class ModelRunner:
         if saved <= 0 or ops.shared_keys_pay_bytes == 0:
             return runs if saved > 0 else None
         return runs if self._reads_once and ops.prefix_keys_pay(runs, self._kv_dtype, longest) and ops.shared_keys_pay(saved * self._key_bytes, longest) else None
+
+    def _send_runs(self, values: List[int]) -> torch.Tensor:
+        self._runs_staging.take(len(values))[: len(values)] = values
+        return self._runs_staging.send(len(values))
 
     def _adapted(self, rids) -> bool:
         return bool(self.adapter_of) and any(rid in self.adapter_of for rid in rids)

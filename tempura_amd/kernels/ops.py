@@ -1560,9 +1560,10 @@ prefix_scratch_limit = 1 << 30
 class SharedKeys:
     """Which requests of a step begin with the same keys: the batch's requests in runs of ``counts[g]`` neighbours, the first
     ``lengths[g]`` keys of every request of run g lying in the same pages (0: they share nothing).  Requests behind the last
-    run (``requests``: how many there are in all) share nothing.  Host lists; made once for as long as the runs stay as they are."""
+    run (``requests``: how many there are in all) share nothing.  Host lists; made once for as long as the runs stay as they are.
+    ``send``: what brings the list of int32 that the kernels read to the device (None: a copy that waits for what is queued on the stream)."""
 
-    def __init__(self, counts, lengths, device, requests: Optional[int] = None):
+    def __init__(self, counts, lengths, device, requests: Optional[int] = None, send=None):
         counts, lengths = [int(c) for c in counts], [int(v) for v in lengths]
         _need(len(counts) == len(lengths), "SharedKeys: one length for every run of requests")
         _need(all(c >= 0 for c in counts) and all(0 <= v < 2 ** 31 for v in lengths), "SharedKeys: counts and lengths must not be negative")
@@ -1581,7 +1582,8 @@ class SharedKeys:
         self.max_requests = max((c for c, v in runs if v), default=0)
         self.sharing = sum(1 for _, v in runs if v)
         self._runs, self._plans, self._bound = [(c, v) for c, v in runs if v], {}, False
-        data = torch.tensor(starts + [v for _, v in runs] + [v for c, v in runs for _ in range(c)], dtype=torch.int32).to(device)
+        values = starts + [v for _, v in runs] + [v for c, v in runs for _ in range(c)]
+        data = torch.tensor(values, dtype=torch.int32).to(device) if send is None else send(values)
         self.starts, self.keys, self.each = data[: self.groups + 1], data[self.groups + 1: 2 * self.groups + 1], data[2 * self.groups + 1:]
 
     def _keep(self, key: tuple, plan) -> None:

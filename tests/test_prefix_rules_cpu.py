@@ -106,3 +106,23 @@ def test_the_engine_and_the_operator_ask_the_same(launched, tiny_dirs):
             rids = [(keys, i) for i in range(3)]
             assert runner._shared_runs(rids) == ([(3, keys)] if sizes and enough else None)
             assert (runner._shared_bounds(rids) is not None) == (sizes and enough)
+
+
+def test_runs_of_eager_steps_travel_like_their_other_inputs(tiny_dirs, monkeypatch):
+    """New runs of requests go to the device through the runner's ring of pinned buffers: the host does not wait for the steps in flight."""
+    from tempura_amd.engine import Engine
+    from tempura_amd.kernels import ops
+    monkeypatch.setattr(ops, "shared_keys_pay_bytes", 0)
+    runner = Engine(tiny_dirs.path("A", "float32"), dtype="float32", device="cpu", page_size=16, kv_pages=256, max_batch_size=8, max_prefixes=1).runner
+    cache, sent, real = runner.cache, [], runner._runs_staging.send
+    cache.add("d"), cache.reserve("d", 64), cache.commit("d", 64)
+    for i in range(4):
+        cache.add(i), cache.share(i, "d", 64)
+    runner._runs_staging.send = lambda n: (sent.append(n), real(n))[1]
+    monkeypatch.setattr(ops.torch, "tensor", lambda *a, **kw: pytest.fail("a copy that waits"))
+    from tempura_amd.engine.runner import StepEntry
+    for rids in ([0, 1], [0, 1, 2], [0, 1]):
+        _, ctx = runner._pack_step([StepEntry(i, [5], [0]) for i in rids])
+        n = len(rids)
+        assert ctx.shared_keys.starts.tolist() == [0, n] and ctx.shared_keys.keys.tolist() == [64] and ctx.shared_keys.each.tolist() == [64] * n
+    assert sent == [2 + 1 + 2, 2 + 1 + 3]       # (the third step's runs are the first's, which are there)
