@@ -1646,7 +1646,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     new tokens among them (a bound, at least the longest; None: ``max_context_len``).  Every row of q belongs to
     a request, whose index in the batch ``token_req`` gives.  Sizes that the kernel is not built for
     (``prefix_attention_ok``), steps without shared keys or with few (``prefix_least_keys``), and portions beside requests with many keys of
-    their own (``prefix_own_steps``) run ``paged_attention``, which gets ``step`` as its ``shared``."""
+    their own (``prefix_own_steps``) run ``paged_attention``, which gets ``step`` as its ``shared``.  Caches
+    that are not aligned to 16 bytes, which whole pieces of them are loaded by, are refused."""
     if _backend is not None:
         return _backend.prefix_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, shared, max_q_len,
                                          max_context_len, max_own_len, num_single, sink, softcap)
@@ -1672,6 +1673,8 @@ def prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if sizes is None:
         return paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens, context_lens, token_req, scale, 0, max_q_len, max_context_len,
                                num_single, sink=sink, softcap=softcap, shared=step)
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise KernelError("prefix_attention: the caches must be aligned to 16 bytes")
     out = q.new_empty((n, heads * q.shape[2]))
     if n == 0:
         return out

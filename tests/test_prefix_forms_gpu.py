@@ -123,3 +123,18 @@ def test_the_same_call_gives_the_same_bits(monkeypatch, form, dtype):
     s = P.step([(9, 640)], [1 + (61 * i) % 200 for i in range(9)], [1, 4, 1, 9, 1, 1, 30, 1, 2], 8, 2, 128, 16, dtype, seed=2)
     first = run(monkeypatch, s, form, 3, 2)
     assert all(torch.equal(run(monkeypatch, s, form, 3, 2), first) for _ in range(3))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_queries_at_odd_places(monkeypatch, dtype):
+    """q may lie anywhere that an element may: the same bits as from an aligned place."""
+    from tempura_amd.kernels import ops
+    monkeypatch.setattr(ops, "prefix_least_keys", (0, 0, 0))
+    s = P.step([(5, 320)], [1, 40, 64, 100, 7], [1, 3, 1, 1, 2], 8, 2, 64, 16, dtype, seed=4)
+    t = {name: s[name].to(DEV) for name in ("q", "k", "v", "tables", "starts", "ctx", "req")}
+    shared = ops.SharedKeys(s["counts"], s["lens"], DEV)
+    call = lambda q: ops.prefix_attention(q, t["k"], t["v"], t["tables"], t["starts"], t["ctx"], t["req"], s["scale"], shared, 3,  # noqa: E731
+                                          int(s["ctx"].max()), max_own_len=s["own"])
+    odd = torch.empty(t["q"].numel() + 1, dtype=dtype, device=DEV)[1:].view(t["q"].shape)
+    odd.copy_(t["q"])
+    assert odd.data_ptr() % 16 and torch.equal(call(odd), call(t["q"]))

@@ -126,3 +126,22 @@ def test_runs_of_eager_steps_travel_like_their_other_inputs(tiny_dirs, monkeypat
         n = len(rids)
         assert ctx.shared_keys.starts.tolist() == [0, n] and ctx.shared_keys.keys.tolist() == [64] and ctx.shared_keys.each.tolist() == [64] * n
     assert sent == [2 + 1 + 2, 2 + 1 + 3]       # (the third step's runs are the first's, which are there)
+
+
+def test_caches_at_odd_places_are_refused(launched):
+    """Keys and values go to LDS in pieces of 16 bytes from where they lie."""
+    from tempura_amd.kernels import ops
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    shared, q = ops.SharedKeys([3], [1024], "cpu"), torch.empty(3, 4, 64, dtype=torch.bfloat16)
+
+    def call(offset_k, offset_v, q=q):
+        k, v = (torch.empty(2 * 2 * 16 * 64 + 8, dtype=torch.bfloat16)[o: o + 2 * 2 * 16 * 64] for o in (offset_k, offset_v))
+        return ops.prefix_attention(q, k.view(2, 2, 16, 64), v.view(2, 2, 64, 16), torch.zeros(3, 70, dtype=torch.int32), i32(0, 1, 2, 3), i32(1030, 1031, 1032),
+                                    i32(0, 1, 2), 0.125, shared, 1, 1032, max_own_len=8)
+    for k, v in ((1, 0), (0, 4), (4, 4), (2, 6)):
+        with pytest.raises(ops.KernelError, match="16 bytes"):
+            call(k, v)
+    assert not launched
+    call(8, 0)
+    call(0, 0, torch.empty(3 * 4 * 64 + 1, dtype=torch.bfloat16)[1:].view(3, 4, 64))       # (q is read with ordinary loads, from anywhere)
+    assert [name for name, _ in launched] == ["tp_prefix_attention"] * 2
