@@ -300,7 +300,7 @@ __device__ inline void prefix_odd_values(const PartRows& w, int j0, int g, const
     for (int t = 0; t < VF; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) odd |= ((vv[dt][t][e] & EXP) + STEP) & TOP;
-  if (__builtin_amdgcn_ballot_w64(odd != 0) == 0) return;
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(odd != 0) == 0, 1)) return;
   auto all = [](unsigned n) { return 0u - min(n, 1u); };      // all bits, unless n is 0
   constexpr unsigned ONE = 0x3f80u, MINUS = 0x4280u, NONE = 0x4580u;      // 1, 64 and 4,096: the upper halves of their float32 bits
   pa_u32x4 sees[NQ][VF];
@@ -602,6 +602,12 @@ __device__ inline void prefix_part_rows(const PrefixArgs& a, unsigned char* stag
     L::arrived(vv);
     if (j0 + 32 > w.end) prefix_clear<E, DT, VF>(w.end, j0, g, vv);
     if (OWN && w.limit0 < j0 + 31) prefix_odd_values<E, NQ, DT, VF>(w, j0, g, limit, vv, o);
+    if constexpr (OWN && E == 2) {      // (both ways here end in the same registers: else every step copies the sums)
+#pragma unroll
+      for (int nq = 0; nq < NQ; ++nq)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) asm volatile("" : "+v"(o[nq][dt]));
+    }
     prefix_values<E, NQ, DT, VF>(vv, pf, o);
   }
   PA_WAIT_VM(0);       // (nothing is on its way into LDS when the block ends)
