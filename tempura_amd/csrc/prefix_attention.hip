@@ -289,7 +289,8 @@ __device__ inline void prefix_values(const pa_u32x4 (&vv)[DT][VF], const pa_u32x
 // Where a row may not see all of the step's keys a value that is not finite has to stay away from the rows in front of it (0 * Inf and 0 * NaN are not 0).  If there is
 // one, which portions of numbers never have, zeros take the place of such values, and the sums get what they would have brought: a product counts for each row and
 // element those that the row sees, 1 for a positive infinity, 64 for a negative one and 4,096 for what is no number (at most 32 of each: exact).  (In integer
-// arithmetic: comparisons' masks would take the scalar registers that the steps' addresses live in.)
+// arithmetic: comparisons' masks would take the scalar registers that the steps' addresses live in.  Steps of numbers pay the check: 6,240 rows behind 6,000 keys 43.7 -> 44.0
+// us, 32 single tokens of 1,000 own keys beside a portion of 64 51.6 -> 52.2.)
 template <int E, int NQ, int DT, int VF>
 __device__ inline void prefix_odd_values(const PartRows& w, int j0, int g, const int (&limit)[NQ], pa_u32x4 (&vv)[DT][VF], pa_f32x4 (&o)[NQ][DT]) {
   constexpr unsigned EXP = E == 2 ? 0x7f807f80u : 0x7f800000u, STEP = E == 2 ? 0x00800080u : 0x00800000u, TOP = E == 2 ? 0x80008000u : 0x80000000u;

@@ -1512,12 +1512,12 @@ def attention_rows(rows, col0: int, ctx, group: int, heads: int, kvh: int, dim: 
 
 
 #: the engine's steps of single tokens, and of portions of up to 128, read shared keys once for all where that saves at least so many bytes of keys and
-#: values a layer (0: they leave it to ``prefix_attention``); of longer portions as many times more as they are longer, of portions up to 64 a twelfth.  (Single tokens behind shared keys, 32 heads of
-#: 128 over 8 key heads, bf16, a captured step of four layers with embedding and head, us, once for all / each for itself: 2 requests of 8,192 keys,
-#: 34 MB a layer saved, 545 / 542; 4 of 4,096, 50 MB, 541 / 542; 8 of 2,048, 59 MB, 550 / 553; 16 of 2,048, 126 MB, 629 / 648; 32 of 1,024, 130 MB, 685 / 678;
-#: 8 of 8,192, 235 MB, 570 / 613; 32 of 2,048, 260 MB, 692 / 703; 32 of 8,192, 1,040 MB, 732 / 865; 64 of 8,192, 2,110 MB, 784 / 1,206.  The attention alone of
-#: 4 and 32 tokens behind 2,048 or 8,192 keys beside a prompt of its own: 4 x 2,048 and 64 tokens, 25 MB, 17.7 / 23.0; 4 x 8,192 and 512, 100 MB, 80 / 56;
-#: 32 x 8,192 and 512, 91 / 112, and 2,048, 258 / 152.)
+#: values a layer (0: ``prefix_attention`` alone decides); of longer portions as many times more as they are longer, of portions up to 64 a twelfth.
+#: (Single tokens behind shared keys, 32 heads of 128 over 8 key heads, bf16, a captured step of four layers with embedding and head, us, once for all / each for
+#: itself: 2 requests of 8,192 keys, 34 MB a layer saved, 545 / 542; 4 of 4,096, 50 MB, 541 / 542; 8 of 2,048, 59 MB, 550 / 553; 16 of 2,048, 126 MB,
+#: 629 / 648; 32 of 1,024, 130 MB, 685 / 678; 8 of 8,192, 235 MB, 570 / 613; 32 of 2,048, 260 MB, 692 / 703; 32 of 8,192, 1,040 MB, 732 / 865; 64 of 8,192,
+#: 2,110 MB, 784 / 1,206.  The attention alone of 4 and 32 tokens behind 2,048 or 8,192 keys beside a prompt of its own: 4 x 2,048 and 64 tokens, 25 MB,
+#: 17.7 / 23.0; 4 x 8,192 and 512, 100 MB, 80 / 56; 32 x 8,192 and 512, 91 / 112, and 2,048, 258 / 152.)
 shared_keys_pay_bytes = 96 << 20
 
 
