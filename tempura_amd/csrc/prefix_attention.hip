@@ -290,7 +290,8 @@ __device__ inline void prefix_values(const pa_u32x4 (&vv)[DT][VF], const pa_u32x
 // one, which portions of numbers never have, zeros take the place of such values, and the sums get what they would have brought: a product counts for each row and
 // element those that the row sees, 1 for a positive infinity, 64 for a negative one and 4,096 for what is no number (at most 32 of each: exact).  (In integer
 // arithmetic: comparisons' masks would take the scalar registers that the steps' addresses live in.  Steps of numbers pay the check: 6,240 rows behind 6,000 keys 43.7 -> 44.0
-// us, 32 single tokens of 1,000 own keys beside a portion of 64 51.6 -> 52.2.)
+// us, 32 single tokens of 1,000 own keys beside a portion of 64 51.6 -> 52.2, float32
+// 378 -> 393.)
 template <int E, int NQ, int DT, int VF>
 __device__ inline void prefix_odd_values(const PartRows& w, int j0, int g, const int (&limit)[NQ], pa_u32x4 (&vv)[DT][VF], pa_f32x4 (&o)[NQ][DT]) {
   constexpr unsigned EXP = E == 2 ? 0x7f807f80u : 0x7f800000u, STEP = E == 2 ? 0x00800080u : 0x00800000u, TOP = E == 2 ? 0x80008000u : 0x80000000u;
@@ -307,7 +308,6 @@ __device__ inline void prefix_odd_values(const PartRows& w, int j0, int g, const
   pa_u32x4 sees[NQ][VF];
 #pragma unroll
   for (int nq = 0; nq < NQ; ++nq) {
-    __builtin_amdgcn_sched_barrier(0);
     const int from = max(w.first, j0), upto = max(from, min(w.end - 1, limit[nq]) + 1);
     auto seen = [&](int key) { return (unsigned)((from - 1 - key) >> 31) & (unsigned)((key - upto) >> 31) & ONE; };
 #pragma unroll
@@ -327,14 +327,17 @@ __device__ inline void prefix_odd_values(const PartRows& w, int j0, int g, const
   for (int dt = 0; dt < DT; ++dt) {
     pa_u32x4 marks[VF];
 #pragma unroll
-    for (int t = 0; t < VF; ++t)
+    for (int t = 0; t < VF; ++t) {
+      // (one tile behind the other, so that they need no registers beyond those of the steps without such values)
+      asm volatile("" : "+v"(vv[dt][t]));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        __builtin_amdgcn_sched_barrier(0);      // (one behind the other: no registers beyond those of the steps without such values)
         const unsigned v = vv[dt][t][e], hi = mark(v >> 16, E == 4 ? v & 0xffffu : 0u), lo = E == 2 ? mark(v & 0xffffu, 0u) : 0u;
         marks[t][e] = hi << 16 | lo;
         vv[dt][t][e] = v & ~(E == 2 ? (all(hi) & 0xffff0000u) | (all(lo) & 0x0000ffffu) : all(hi));
       }
+      asm volatile("" : "+v"(vv[dt][t]), "+v"(marks[t]));
+    }
 #pragma unroll
     for (int nq = 0; nq < NQ; ++nq) {
       pa_f32x4 count = {0.f, 0.f, 0.f, 0.f};
@@ -801,9 +804,10 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(const float* __restric
   else from_float4((float*)out + to, acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
+// (two blocks a CU where LDS holds two, but for float32 blocks of 128 rows, whose registers do not)
 template <int E, int D, int NQS, int NSS, int NQO, int NSO>
 static int prefix_launch(const PrefixArgs& a, int blocks, hipStream_t s) {
-  prefix_attention_kernel<E, D, NQS, NSS, NQO, NSO, E == 2 ? 2 : 1><<<blocks, PA_WAVES * 64, 0, s>>>(a);
+  prefix_attention_kernel<E, D, NQS, NSS, NQO, NSO, E == 2 || (NQS == 1 && NSO > 0) ? 2 : 1><<<blocks, PA_WAVES * 64, 0, s>>>(a);
   return 0;
 }
 
